@@ -7,8 +7,8 @@ import subprocess
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
-SOURCES = ["api.hip", "siren.hip", "fused.hip", "fused_nodes.hip", "fused_wide.hip", "node.hip", "nodegrad.hip", "trilerp.hip", "loss.hip", "optim.hip"]
-HEADERS = ["common.h", "gemm_engine.h", "fused.h", "fused_dev.h", "nodes.h", "nodegrad.h", "node_device.h", "k1_device.h", "step_device.h", "dw_device.h", "wide_dev.h", "noderows_device.h", "ngprep_device.h", os.path.join("..", "..", "include", "cinema_hip.h")]
+SOURCES = ["api.hip", "siren.hip", "fused.hip", "fused_nodes.hip", "fused_wide.hip", "node.hip", "nodegrad.hip", "trilerp.hip", "loss.hip", "optim.hip", "linear.hip", "layernorm.hip", "gradnorm.hip"]
+HEADERS = ["common.h", "gemm_engine.h", "fused.h", "fused_dev.h", "nodes.h", "nodegrad.h", "node_device.h", "k1_device.h", "step_device.h", "dw_device.h", "wide_dev.h", "noderows_device.h", "ngprep_device.h", "mlp_gemm.h", "rows.h", os.path.join("..", "..", "include", "cinema_hip.h")]
 OUT = os.path.join(_HERE, "libcinema_hip.so")
 
 
@@ -36,7 +36,9 @@ def build(force: bool = False, verbose: bool = True, trace: bool = False) -> str
     # objects whose source and headers are older than they are get reused unless force is set
     objdir = os.path.join(_HERE, "..", "build", "obj_trace" if trace else "obj")
     os.makedirs(objdir, exist_ok=True)
-    flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC"] + (["-DFUSED_TRACE_BUILD"] if trace else [])
+    # no packed fp32 instructions: some of their forms have given wrong results on this hardware
+    flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + \
+        (["-DFUSED_TRACE_BUILD"] if trace else [])
     newest_header = max(os.path.getmtime(os.path.join(CSRC, h)) for h in HEADERS)
     procs, objs = [], []
     for src in SOURCES:

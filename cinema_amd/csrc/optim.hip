@@ -12,6 +12,8 @@ struct AdamArgs {
   cinema_adamw_group g[CINEMA_ADAMW_MAX_GROUPS];
   float bc1[CINEMA_ADAMW_MAX_GROUPS], bc2_rsqrt[CINEMA_ADAMW_MAX_GROUPS];
   int n_groups, clear_grads;
+  const float *norm;   // device: gradient norm of a clipped step, null otherwise
+  float max_norm;
 };
 
 __device__ __forceinline__ void adam_one(float &p, float g, float &m, float &v, const cinema_adamw_group &c, float step_size,
@@ -24,8 +26,14 @@ __device__ __forceinline__ void adam_one(float &p, float g, float &m, float &v, 
   p -= step_size * (m / denom);
 }
 
+template <bool CLIP>
 __global__ __launch_bounds__(256) void k_adamw(AdamArgs a) {
   const cinema_adamw_group c = a.g[blockIdx.y];
+  float scale = 1.f;
+  if (CLIP) {
+    const double ratio = (double)a.max_norm / ((double)a.norm[0] + 1e-6);
+    scale = ratio >= 1. ? 1.f : (float)ratio;      // NaN stays NaN
+  }
   const float step_size = c.lr / a.bc1[blockIdx.y];
   const float r2 = a.bc2_rsqrt[blockIdx.y];
   const long n4 = c.n >> 2;
@@ -40,7 +48,7 @@ __global__ __launch_bounds__(256) void k_adamw(AdamArgs a) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         float pk = p[k], mk = m[k], vk = v[k];
-        adam_one(pk, g[k], mk, vk, c, step_size, r2);
+        adam_one(pk, CLIP ? g[k] * scale : g[k], mk, vk, c, step_size, r2);
         p[k] = pk; m[k] = mk; v[k] = vk;
       }
       reinterpret_cast<f32x4 *>(c.p)[i] = p;
@@ -51,14 +59,14 @@ __global__ __launch_bounds__(256) void k_adamw(AdamArgs a) {
     done = n4 << 2;
   }
   for (long i = done + (long)blockIdx.x * blockDim.x + threadIdx.x; i < c.n; i += (long)gridDim.x * blockDim.x) {
-    adam_one(c.p[i], c.g[i], c.m[i], c.v[i], c, step_size, r2);
+    adam_one(c.p[i], CLIP ? c.g[i] * scale : c.g[i], c.m[i], c.v[i], c, step_size, r2);
     if (a.clear_grads) const_cast<float *>(c.g)[i] = 0.f;
   }
 }
 
 }  // namespace
 
-static int adamw_impl(const cinema_adamw_group *groups, int32_t n_groups, int clear_grads, void *stream) {
+static int adamw_impl(const cinema_adamw_group *groups, int32_t n_groups, int clear_grads, const float *norm, float max_norm, void *stream) {
   CINEMA_REQUIRE(groups != nullptr && n_groups >= 1 && n_groups <= CINEMA_ADAMW_MAX_GROUPS,
                  "cinema_adamw_step: need 1..%d groups", CINEMA_ADAMW_MAX_GROUPS);
   AdamArgs a = {};
@@ -73,17 +81,26 @@ static int adamw_impl(const cinema_adamw_group *groups, int32_t n_groups, int cl
   }
   a.n_groups = n_groups;
   a.clear_grads = clear_grads;
+  a.norm = norm;
+  a.max_norm = max_norm;
   if (nmax == 0) return 0;
   const unsigned gx = (unsigned)std::min<long>((nmax / 4 + 255) / 256 + 1, 2048);
-  hipLaunchKernelGGL(k_adamw, dim3(gx, n_groups), dim3(256), 0, (hipStream_t)stream, a);
+  if (norm != nullptr) hipLaunchKernelGGL(k_adamw<true>, dim3(gx, n_groups), dim3(256), 0, (hipStream_t)stream, a);
+  else hipLaunchKernelGGL(k_adamw<false>, dim3(gx, n_groups), dim3(256), 0, (hipStream_t)stream, a);
   CINEMA_CHECK_HIP(hipGetLastError());
   return 0;
 }
 
 extern "C" int cinema_adamw_step(const cinema_adamw_group *groups, int32_t n_groups, void *stream) {
-  return adamw_impl(groups, n_groups, 0, stream);
+  return adamw_impl(groups, n_groups, 0, nullptr, 0.f, stream);
 }
 
 extern "C" int cinema_adamw_step_clear(const cinema_adamw_group *groups, int32_t n_groups, void *stream) {
-  return adamw_impl(groups, n_groups, 1, stream);
+  return adamw_impl(groups, n_groups, 1, nullptr, 0.f, stream);
+}
+
+extern "C" int cinema_adamw_step_clipped(const cinema_adamw_group *groups, int32_t n_groups, int32_t clear_grads, const float *norm,
+                                         float max_norm, void *stream) {
+  CINEMA_REQUIRE(norm != nullptr, "cinema_adamw_step_clipped: null norm");
+  return adamw_impl(groups, n_groups, clear_grads, norm, max_norm, stream);
 }

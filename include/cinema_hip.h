@@ -491,6 +491,69 @@ int cinema_adamw_step(const cinema_adamw_group *groups /* host */, int32_t n_gro
  * optimizer.zero_grad(), build_atlas.py:82-87, in one pass over the gradient). */
 int cinema_adamw_step_clear(const cinema_adamw_group *groups /* host */, int32_t n_groups, void *stream);
 
+/* -------------------------------------------------------------------------------------
+ * Plain MLP operators beside the sine layers (models/inr_decoder.py:126-141 LatentRegressor; no counterpart of the residual,
+ * the layer norm and the clipping in the reference).  Element types of the row buffers: CINEMA_DT_*; sums, statistics and
+ * epilogues are fp32 or wider, results are rounded once.  Row buffers without a stride argument are contiguous.
+ * ------------------------------------------------------------------------------------- */
+#define CINEMA_DT_F32 0
+#define CINEMA_DT_BF16 1
+#define CINEMA_DT_F16 2
+#define CINEMA_ACT_NONE 0
+#define CINEMA_ACT_RELU 1
+#define CINEMA_ACT_GELU 2      /* 0.5 z (1 + erf(z / sqrt 2)) */
+#define CINEMA_ACT_GELU_TANH 3 /* 0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */
+#define CINEMA_ACT_SILU 4      /* z / (1 + e^-z) */
+
+/* y [M x N] = act(x [M x K, row stride ldx] W [N x K]^T + bias [N]) + res [M x N, row stride ldres]; bias and res may be NULL.
+ * bias is fp32 (bias_f32 != 0) or of the rows' type.  z (NULL if no gradient is wanted): what the backward pass reads of the
+ * pre-activations, [M x N] fp16 for the 16-bit types, fp32 for fp32.  work: cinema_linear_work_bytes(..., 0) bytes (NULL if 0).
+ * 1 <= M < 2^31, 1 <= K, N <= 2^24; cinema_linear_work_bytes returns -1 for anything else. */
+int64_t cinema_linear_work_bytes(int64_t M, int64_t K, int64_t N, int32_t dtype, int32_t backward);
+int cinema_linear_forward(const void *x, int64_t ldx, const void *w, const void *bias, int32_t bias_f32, const void *res,
+                          int64_t ldres, int64_t M, int64_t K, int64_t N, int32_t act, int32_t dtype, void *z, void *y,
+                          void *work, void *stream);
+/* dz = dy * act'(z);  dx [M x K] = dz W,  dw [N x K] = dz^T x,  db [N] = column sums of dz (fp32 if db_f32, else the rows'
+ * type).  dx, dw, db may be NULL.  z may be NULL for CINEMA_ACT_NONE.  The residual's gradient is dy itself.  Every sum has a
+ * fixed order: equal inputs give equal bits.  work: cinema_linear_work_bytes(..., 1) bytes. */
+int cinema_linear_backward(const void *dy, const void *z, const void *x, int64_t ldx, const void *w, int64_t M, int64_t K,
+                           int64_t N, int32_t act, int32_t dtype, int32_t db_f32, void *dx, void *dw, void *db, void *work,
+                           void *stream);
+
+/* Layer norm of rows of D values: y = (x - mean) rstd w + b, rstd = 1 / sqrt(variance + eps); w, b [D] may be NULL, fp32
+ * (w_f32 != 0) or of the rows' type.  mean, rstd [M] fp32: what the backward pass reads (NULL if no gradient is wanted).
+ * Backward: dx [M x D], dw, db [D] (w's type); each may be NULL.  Every sum has a fixed order.
+ * work: cinema_layer_norm_work_bytes bytes, NULL if neither dw nor db is wanted. */
+int64_t cinema_layer_norm_work_bytes(int64_t M, int64_t D, int32_t dtype);
+int cinema_layer_norm_forward(const void *x, int64_t ldx, const void *w, const void *b, int32_t w_f32, int64_t M, int64_t D,
+                              float eps, int32_t dtype, void *y, float *mean, float *rstd, void *stream);
+int cinema_layer_norm_backward(const void *dy, const void *x, int64_t ldx, const void *w, int32_t w_f32, const float *mean,
+                               const float *rstd, int64_t M, int64_t D, int32_t dtype, void *dx, void *dw, void *db,
+                               void *work, void *stream);
+
+/* Global norm of many gradients, and clipping to it (torch.nn.utils.clip_grad_norm_):
+ * norm = (sum |g|^p)^(1/p) over all values of all tensors, kind = p = 1 or 2, kind 0: max |g|; sums in 64 bits, fixed order.
+ * cinema_grad_clip then multiplies every gradient by min(1, max_norm / (norm + 1e-6)) in place; nothing is written where that
+ * is 1.  A NaN norm gives NaN gradients, an infinite one zeros (NaN where the gradient is infinite).  The tensors are
+ * contiguous and do not overlap.  norm: one device float, the norm before clipping.
+ * work: cinema_grad_norm_work_bytes(number of tensors) bytes. */
+typedef struct cinema_grad_tensor {
+  void *g;       /* device */
+  int64_t n;     /* values */
+  int32_t dtype; /* CINEMA_DT_* */
+  int32_t reserved;
+} cinema_grad_tensor;
+
+int64_t cinema_grad_norm_work_bytes(int64_t n_tensors);
+int cinema_grad_norm(const cinema_grad_tensor *tensors /* host */, int32_t n, int32_t kind, void *work, float *norm,
+                     void *stream);
+int cinema_grad_clip(const cinema_grad_tensor *tensors /* host */, int32_t n, int32_t kind, float max_norm, void *work,
+                     float *norm, void *stream);
+/* cinema_adamw_step / _clear on gradients multiplied by min(1, max_norm / (norm[0] + 1e-6)) on the way; norm: a device float,
+ * as cinema_grad_norm leaves it.  The gradients themselves stay as they are (or are zeroed, clear_grads != 0). */
+int cinema_adamw_step_clipped(const cinema_adamw_group *groups /* host */, int32_t n_groups, int32_t clear_grads,
+                              const float *norm, float max_norm, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
