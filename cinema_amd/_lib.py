@@ -142,6 +142,24 @@ def load():
     return lib
 
 
+_binding = None
+
+
+def binding():
+    """The extension module of the plain MLP operators (csrc/binding.cpp), bound to this library once."""
+    global _binding
+    if _binding is None:
+        load()
+        try:
+            from . import _binding as mod
+        except ImportError as e:
+            raise CinemaHipError(f"cinema_amd/_binding.so is missing or does not load ({e}): build it with "
+                                 "`python -c 'import __graft_entry__ as g; g.build()'`") from e
+        mod.bind(LIB_PATH, CinemaHipError)
+        _binding = mod
+    return _binding
+
+
 def check(rc: int, what: str = ""):
     if rc != 0:
         msg = load().cinema_last_error()

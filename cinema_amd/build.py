@@ -4,12 +4,14 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+import sysconfig
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
 SOURCES = ["api.hip", "siren.hip", "fused.hip", "fused_nodes.hip", "fused_wide.hip", "node.hip", "nodegrad.hip", "trilerp.hip", "loss.hip", "optim.hip", "linear.hip", "layernorm.hip", "gradnorm.hip"]
 HEADERS = ["common.h", "gemm_engine.h", "fused.h", "fused_dev.h", "nodes.h", "nodegrad.h", "node_device.h", "k1_device.h", "step_device.h", "dw_device.h", "wide_dev.h", "noderows_device.h", "ngprep_device.h", "mlp_gemm.h", "rows.h", os.path.join("..", "..", "include", "cinema_hip.h")]
 OUT = os.path.join(_HERE, "libcinema_hip.so")
+BINDING_SOURCE, BINDING = "binding.cpp", os.path.join(_HERE, "_binding.so")
 
 
 def _hipcc() -> str:
@@ -20,10 +22,21 @@ def _hipcc() -> str:
 
 
 def needs_build() -> bool:
-    if not os.path.exists(OUT):
+    if not os.path.exists(OUT) or not os.path.exists(BINDING):
         return True
     t = os.path.getmtime(OUT)
-    return any(os.path.getmtime(os.path.join(CSRC, f)) > t for f in SOURCES + HEADERS)
+    return any(os.path.getmtime(os.path.join(CSRC, f)) > t for f in SOURCES + HEADERS) or \
+        any(os.path.getmtime(os.path.join(CSRC, f)) > os.path.getmtime(BINDING) for f in (BINDING_SOURCE, HEADERS[-1]))
+
+
+def _binding_command():
+    """Host code against torch's headers (g++): argument checks and autograd nodes of the plain MLP operators."""
+    from torch.utils import cpp_extension as ext
+    torch_paths = [p for p in ext.include_paths("cuda")]
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_binding",
+            "-DTORCH_API_INCLUDE_EXTENSION_H"] + [f"-I{p}" for p in torch_paths + [sysconfig.get_paths()["include"]]] + \
+        [BINDING_SOURCE, "-o", BINDING] + [f"-L{p}" for p in ext.library_paths("cuda") if os.path.isdir(p)] + \
+        ["-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-ldl"]
 
 
 def build(force: bool = False, verbose: bool = True, trace: bool = False) -> str:
@@ -41,6 +54,11 @@ def build(force: bool = False, verbose: bool = True, trace: bool = False) -> str
         (["-DFUSED_TRACE_BUILD"] if trace else [])
     newest_header = max(os.path.getmtime(os.path.join(CSRC, h)) for h in HEADERS)
     procs, objs = [], []
+    if not trace:
+        cmd = _binding_command()
+        if verbose:
+            print("[cinema_amd.build]", " ".join(cmd), flush=True)
+        procs.append((cmd, subprocess.Popen(cmd, cwd=CSRC)))
     for src in SOURCES:
         obj = os.path.join(objdir, src.replace(".hip", ".o"))
         objs.append(obj)

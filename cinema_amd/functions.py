@@ -254,164 +254,3 @@ class ConvModFunction(torch.autograd.Function):
                                                 _lib.ptr(ctx.work), _lib.ptr(din), _lib.ptr(dw), _lib.ptr(db), stream),
                    "cinema_conv_mod_backward")
         return din, dw, db, None
-
-
-# ---- plain MLP operators (models/mlp.py) -----------------------------------------------------------------------------------
-DTYPES = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
-
-
-class _OnDevice:
-    """Makes `device` current for a launch if it is not (a kernel goes to the device that is current at the call)."""
-
-    def __init__(self, device):
-        self.ctx = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *a):
-        if self.ctx is not None:
-            self.ctx.__exit__(*a)
-
-
-def _first_order_only(what: str):
-    """A backward pass under create_graph=True: its results would silently carry no graph."""
-    if torch.is_grad_enabled():
-        raise RuntimeError(f"cinema_amd {what}: the gradients have no second derivative (create_graph=True)")
-
-
-def _raw_stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-def _work(nbytes: int, device, what: str):
-    if nbytes < 0:
-        _lib.check(-1, what)
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-
-
-def _p(t):
-    return None if t is None else t.data_ptr()
-
-
-def _row_major(x2):
-    """(x2 or its contiguous copy, row stride in elements) for the kernels: rows contiguous, any stride of at least a row."""
-    m, k = x2.shape
-    if (x2.stride(1) != 1 and k > 1) or (x2.stride(0) < k and m > 1):
-        x2 = x2.contiguous()
-    return x2, (x2.stride(0) if m > 1 else k)
-
-
-def linear_act_forward(x2, w, bias, res2, act: int, keep: bool):
-    """(y, z) of contiguous w and 2-d rows; z is None unless `keep` and there is an activation."""
-    lib = _lib.load()
-    (m, k), n, dev = x2.shape, w.shape[0], x2.device
-    y = torch.empty((m, n), dtype=x2.dtype, device=dev)
-    z = torch.empty((m, n), dtype=torch.float32 if x2.dtype == torch.float32 else torch.float16, device=dev) if keep and act else None
-    if m == 0:
-        return y, z
-    x2, ldx = _row_major(x2)
-    ldr = 0
-    if res2 is not None:
-        res2, ldr = _row_major(res2)
-    dt = DTYPES[x2.dtype]
-    with _OnDevice(dev):
-        work = _work(lib.cinema_linear_work_bytes(m, k, n, dt, 0), dev, "cinema_linear_work_bytes")
-        rc = lib.cinema_linear_forward(x2.data_ptr(), ldx, w.data_ptr(), _p(bias), int(bias is not None and bias.dtype == torch.float32),
-                                       _p(res2), ldr, m, k, n, act, dt, _p(z), y.data_ptr(), _p(work), _raw_stream(dev))
-    _lib.check(rc, "cinema_linear_forward")
-    return y, z
-
-
-class LinearActFunction(torch.autograd.Function):
-    """y = act(x W^T + b) + r as one node (cinema_linear_forward / _backward).  Kept for the backward pass: x, W and, with an
-    activation, the pre-activations (fp16 for 16-bit rows, fp32 for fp32)."""
-
-    @staticmethod
-    def forward(ctx, x2, w, bias, res2, act: int):
-        need = ctx.needs_input_grad
-        y, z = linear_act_forward(x2, w, bias, res2, act, need[0] or need[1] or need[2])
-        ctx.save_for_backward(x2 if need[1] else None, w if need[0] else None, z)
-        ctx.act, ctx.shape = act, (x2.shape[0], x2.shape[1], w.shape[0])
-        ctx.bias_dtype = None if bias is None else bias.dtype
-        return y
-
-    @staticmethod
-    def backward(ctx, gout):
-        _first_order_only("linear_act")
-        need = ctx.needs_input_grad
-        x2, w, z = ctx.saved_tensors
-        m, k, n = ctx.shape
-        dev = gout.device
-        if not (need[0] or need[1] or need[2]):
-            return None, None, None, gout, None
-        new = torch.zeros if m == 0 else torch.empty
-        dx = new((m, k), dtype=gout.dtype, device=dev) if need[0] else None
-        dw = new((n, k), dtype=gout.dtype, device=dev) if need[1] else None
-        db = new((n,), dtype=ctx.bias_dtype, device=dev) if need[2] else None
-        if m:
-            lib = _lib.load()
-            g = gout.contiguous()
-            ldx = k
-            if x2 is not None:
-                x2, ldx = _row_major(x2)
-            dt = DTYPES[g.dtype]
-            with _OnDevice(dev):
-                work = _work(lib.cinema_linear_work_bytes(m, k, n, dt, 1), dev, "cinema_linear_work_bytes")
-                rc = lib.cinema_linear_backward(g.data_ptr(), _p(z), _p(x2), ldx, _p(w), m, k, n, ctx.act, dt,
-                                                int(ctx.bias_dtype == torch.float32), _p(dx), _p(dw), _p(db), _p(work), _raw_stream(dev))
-            _lib.check(rc, "cinema_linear_backward")
-        return dx, dw, db, gout if need[3] else None, None
-
-
-def layer_norm_forward(x2, w, b, eps: float, keep: bool):
-    """(y, mean, rstd) of 2-d rows; the statistics are None unless `keep`."""
-    lib = _lib.load()
-    (m, d), dev = x2.shape, x2.device
-    y = torch.empty((m, d), dtype=x2.dtype, device=dev)
-    mean, rstd = torch.empty((2, m), dtype=torch.float32, device=dev).unbind(0) if keep else (None, None)
-    if m == 0:
-        return y, mean, rstd
-    x2, ldx = _row_major(x2)
-    wt = w if w is not None else b
-    with _OnDevice(dev):
-        rc = lib.cinema_layer_norm_forward(x2.data_ptr(), ldx, _p(w), _p(b), int(wt is not None and wt.dtype == torch.float32), m, d, eps,
-                                           DTYPES[x2.dtype], y.data_ptr(), _p(mean), _p(rstd), _raw_stream(dev))
-    _lib.check(rc, "cinema_layer_norm_forward")
-    return y, mean, rstd
-
-
-class LayerNormFunction(torch.autograd.Function):
-    """Layer norm over the last dimension as one node (cinema_layer_norm_forward / _backward).  Kept: x, w, the statistics."""
-
-    @staticmethod
-    def forward(ctx, x2, w, b, eps: float):
-        y, mean, rstd = layer_norm_forward(x2, w, b, eps, True)
-        ctx.save_for_backward(x2, w, mean, rstd)
-        ctx.w_dtype = w.dtype if w is not None else (b.dtype if b is not None else x2.dtype)
-        return y
-
-    @staticmethod
-    def backward(ctx, gout):
-        _first_order_only("layer_norm")
-        need = ctx.needs_input_grad
-        x2, w, mean, rstd = ctx.saved_tensors
-        (m, d), dev = x2.shape, gout.device
-        new = torch.zeros if m == 0 else torch.empty
-        dx = new((m, d), dtype=x2.dtype, device=dev) if need[0] else None
-        dw = new((d,), dtype=ctx.w_dtype, device=dev) if need[1] else None
-        db = new((d,), dtype=ctx.w_dtype, device=dev) if need[2] else None
-        if m:
-            lib = _lib.load()
-            g = gout.contiguous()
-            x2, ldx = _row_major(x2)
-            dt = DTYPES[x2.dtype]
-            with _OnDevice(dev):
-                work = None
-                if need[1] or need[2]:
-                    work = _work(lib.cinema_layer_norm_work_bytes(m, d, dt), dev, "cinema_layer_norm_work_bytes")
-                rc = lib.cinema_layer_norm_backward(g.data_ptr(), x2.data_ptr(), ldx, _p(w), int(ctx.w_dtype == torch.float32), mean.data_ptr(),
-                                                    rstd.data_ptr(), m, d, dt, _p(dx), _p(dw), _p(db), _p(work), _raw_stream(dev))
-            _lib.check(rc, "cinema_layer_norm_backward")
-        return dx, dw, db, None
