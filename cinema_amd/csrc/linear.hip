@@ -12,55 +12,107 @@ namespace {
 
 enum { ACT_NONE = 0, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU, ACT_COUNT };
 
-// 16-bit types take the hardware exponential and reciprocal (about 1e-6 relative, under a four-hundredth of their rounding)
-template <bool FAST> __device__ __forceinline__ float exp_(float x) { return FAST ? __expf(x) : expf(x); }
-template <bool FAST> __device__ __forceinline__ float div_(float a, float b) { return FAST ? a * __builtin_amdgcn_rcpf(b) : a / b; }
+// 16-bit types: the hardware's 2^x and 1/x (1 ulp each, a few 1e-7 relative in what follows, against 2^-8 or 2^-11 of the
+// rounding); a value costs 11 (silu) to 20 (gelu) vector slots, erff alone about 40, which on 25000 x 512 would be a third of
+// the kernel's time.  fp32: the library's functions and true divisions.
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float rcp_hw(float x) { return __builtin_amdgcn_rcpf(x); }
+__device__ __forceinline__ float sigmoid_hw(float x) { return rcp_hw(1.f + exp2_hw(x * -1.4426950408889634f)); }
+__device__ __forceinline__ float within(float z, float m) { return __builtin_amdgcn_fmed3f(z, -m, m); }
 
-template <bool FAST>
-__device__ __forceinline__ float act_value(float z, int act) {
+// P(N(0, 1) > |z|) and e^(-z^2/2): erfc by Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26 (absolute error
+// 1.5e-7)
+__device__ __forceinline__ float normal_tail_hw(float z, float &e) {
+  const float t = rcp_hw(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.f));
+  float p = fmaf(t, 1.061405429f * 0.5f, -1.453152027f * 0.5f);
+  p = fmaf(t, p, 1.421413741f * 0.5f);
+  p = fmaf(t, p, -0.284496736f * 0.5f);
+  p = fmaf(t, p, 0.254829592f * 0.5f) * t;
+  e = exp2_hw(z * z * (-0.5f * 1.4426950408889634f));
+  return p * e;
+}
+constexpr float TANH_A = 0.79788456080286536f;      // sqrt(2 / pi)
+
+// act(z) of eight values; NaN stays
+template <bool HW>
+__device__ __forceinline__ void act8(float (&v)[8], int act) {
   switch (act) {
-    case ACT_RELU: return z < 0.f ? 0.f : z;                                      // NaN stays
-    case ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    case ACT_GELU_TANH: {                                                         // 0.5 z (1 + tanh u) = z / (1 + e^-2u)
-      const float u = 0.79788456080286536f * (z + 0.044715f * z * z * z);
-      return div_<FAST>(z, 1.f + exp_<FAST>(-2.f * u));
-    }
-    case ACT_SILU: return div_<FAST>(z, 1.f + exp_<FAST>(-z));
-    default: return z;
+    case ACT_RELU:
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = v[k] < 0.f ? 0.f : v[k];
+      break;
+    case ACT_GELU:
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        float e;
+        const float z = v[k];
+        // z q for z < 0, z - z q for z > 0, q the small side's probability; infinities: q is 0 there
+        if (HW) v[k] = fmaf(-fminf(fabsf(z), 60.f), normal_tail_hw(z, e), fmaxf(z, 0.f));
+        else v[k] *= 0.5f * (1.f + erff(z * 0.70710678118654752f));
+      }
+      break;
+    case ACT_GELU_TANH:                             // 0.5 z (1 + tanh u) = z / (1 + e^-2u)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float z = v[k], u2 = z * fmaf(2.f * TANH_A * 0.044715f, z * z, 2.f * TANH_A);
+        v[k] = HW ? z * sigmoid_hw(u2) : z / (1.f + expf(-u2));
+      }
+      break;
+    case ACT_SILU:
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = HW ? v[k] * sigmoid_hw(v[k]) : v[k] / (1.f + expf(-v[k]));
+      break;
+    default: break;
   }
 }
 
-template <bool FAST>
-__device__ __forceinline__ float act_slope(float z, int act) {
+// g * act'(z) of eight values.  The factors of z beyond which act' has its limit are bounded: 0 * infinity otherwise.
+template <bool HW>
+__device__ __forceinline__ void slope8(float (&g)[8], const float (&zs)[8], int act) {
   switch (act) {
-    case ACT_RELU: return z <= 0.f ? 0.f : 1.f;
-    case ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * exp_<FAST>(-0.5f * z * z);
-    case ACT_GELU_TANH: {
-      const float z2 = z * z;
-      if (z2 > 400.f) return z > 0.f ? 1.f : 0.f;                                 // s (1 - s) is 0 there, its factor may overflow
-      const float u = 0.79788456080286536f * (z + 0.044715f * z * z2);
-      const float s = div_<FAST>(1.f, 1.f + exp_<FAST>(-2.f * u));
-      return s + z * 2.f * s * (1.f - s) * 0.79788456080286536f * (1.f + 0.134145f * z2);
-    }
-    case ACT_SILU: {
-      if (z < -80.f) return 0.f;                                                  // below fp32's least value; e^-z would overflow
-      const float s = div_<FAST>(1.f, 1.f + exp_<FAST>(-z));
-      return s * (1.f + z * (1.f - s));
-    }
-    default: return 1.f;
+    case ACT_RELU:                                  // the kept value is the slope
+#pragma unroll
+      for (int k = 0; k < 8; ++k) g[k] *= zs[k];
+      break;
+    case ACT_GELU:
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float z = zs[k];
+        float e, c;
+        if (HW) {
+          const float q = normal_tail_hw(z, e);
+          c = z < 0.f ? q : 1.f - q;
+        } else {
+          c = 0.5f * (1.f + erff(z * 0.70710678118654752f));
+          e = expf(-0.5f * z * z);
+        }
+        g[k] *= fmaf(within(z, 60.f) * 0.39894228040143268f, e, c);
+      }
+      break;
+    case ACT_GELU_TANH:
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float z = zs[k], u2 = z * fmaf(2.f * TANH_A * 0.044715f, z * z, 2.f * TANH_A), b = within(z, 60.f);
+        const float s = HW ? sigmoid_hw(u2) : 1.f / (1.f + expf(-u2));
+        g[k] *= fmaf(b * (2.f * TANH_A) * fmaf(0.134145f * b, b, 1.f), s * (1.f - s), s);
+      }
+      break;
+    case ACT_SILU:
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float s = HW ? sigmoid_hw(zs[k]) : 1.f / (1.f + expf(-zs[k]));
+        g[k] *= s * fmaf(within(zs[k], 120.f), 1.f - s, 1.f);
+      }
+      break;
+    default: break;
   }
 }
 
-// what is kept of z: fp16 for the 16-bit types, clamped to its range; a z that fp16 cannot tell from 0 keeps its sign (relu)
+// what is kept of z for the backward pass: fp16 for the 16-bit types (infinite beyond its range, where act' has its limit), fp32
+// for fp32; of relu the slope itself, which no rounding of a small z can turn
 template <typename T> struct Kept { typedef f16_t type; };
 template <> struct Kept<float> { typedef float type; };
-__device__ __forceinline__ void keep(float z, float &d) { d = z; }
-__device__ __forceinline__ void keep(float z, f16_t &d) {
-  const float c = z > 65504.f ? 65504.f : (z < -65504.f ? -65504.f : z);
-  f16_t h = (f16_t)c;
-  if ((float)h == 0.f && c != 0.f) h = c > 0.f ? (f16_t)5.9604645e-8f : (f16_t)-5.9604645e-8f;
-  d = h;
-}
+__device__ __forceinline__ float kept_value(float z, int act) { return act == ACT_RELU ? (z <= 0.f ? 0.f : (z > 0.f ? 1.f : z)) : z; }
 
 template <typename S>
 __device__ __forceinline__ void load8(const S *p, int n, float (&v)[8]) {
@@ -110,38 +162,91 @@ __device__ __forceinline__ void load_bias(const Epilogue &e, int64_t j, int n, f
   }
 }
 
-// eight results of row i, columns j .. j + n - 1
+// eight sums of row i, columns j .. j + n - 1, the bias in them; r: the residual's values
 template <typename T>
-__device__ __forceinline__ void finish8(const Epilogue &e, int64_t i, int64_t j, int n, int64_t J, float (&v)[8], const float (&b)[8]) {
+__device__ __forceinline__ void finish8(const Epilogue &e, int64_t i, int64_t j, int n, int64_t J, float (&v)[8], const float (&r)[8]) {
   typedef typename Kept<T>::type Z;
-  constexpr bool FAST = sizeof(T) == 2;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] += b[k];
   if (e.z != nullptr) {
-    Z h[8];
+    float h[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) keep(v[k], h[k]);
-    Z *zp = (Z *)e.z + i * J + j;
-    if (n >= 8) __builtin_memcpy(zp, h, sizeof(h));
-    else
-      for (int k = 0; k < 8; ++k)
-        if (k < n) zp[k] = h[k];
+    for (int k = 0; k < 8; ++k) h[k] = kept_value(v[k], e.act);
+    store8((Z *)e.z + i * J + j, n, h);
   }
-#pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = act_value<FAST>(v[k], e.act);
+  act8<sizeof(T) == 2>(v, e.act);
   if (e.res != nullptr) {
-    float r[8];
-    load8((const T *)e.res + i * e.ldres + j, n, r);
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] += r[k];
   }
   store8((T *)e.out + i * J + j, n, v);
 }
 
-// One workgroup = one BI x BJ tile of one split.  The results leave through LDS (32 x BJ/WJ values per wave at a time): the
-// matrix unit's layout puts a row's neighbours into different lanes, the epilogue wants eight of them in one.
+// The results leave through LDS (32 x BJ/WJ values per wave at a time): the matrix unit's layout puts a row's neighbours into
+// different lanes, the epilogue wants eight of them in one.  FULL: no row or column of the tile is past the end.
+template <typename T, int BI, int BJ, int WI, int WJ, typename G, bool FULL>
+__device__ __forceinline__ void write_tile(const f32x16 (&acc)[G::TI][G::TJ], int64_t I, int64_t J, const Epilogue &e, int64_t i0, int64_t j0,
+                                           char *smem, int lane, int wave) {
+  constexpr int WTI = BI / WI, WTJ = BJ / WJ, PER = WTJ / 8, RPP = 64 / PER;   // lanes per row, rows per pass
+  constexpr int PASSES = 32 / RPP;
+  static_assert(WI * WJ * 32 * WTJ * 4 <= G::SMEM && (WTJ == 64 || WTJ == 32), "the slabs fit the buffers");
+  LDS_AS float *slab = (LDS_AS float *)(lds_char *)smem + wave * 32 * WTJ;
+  // 16-byte chunk c of slab row r sits in slot c ^ slot_key(r): neither the 64 lanes of a write nor 16 lanes of a read meet a bank twice
+  auto slot_key = [](int r) { return WTJ == 64 ? (r & 1) | (((r >> 2) & 1) << 3) : (r >> 1) & 1; };
+  const int c8 = (lane % PER) * 8;
+  const int64_t j = j0 + (wave % WJ) * WTJ + c8;
+  const int n = FULL ? 8 : (j >= J ? 0 : (J - j < 8 ? (int)(J - j) : 8));
+#pragma unroll
+  for (int x = 0; x < G::TI; ++x) {
+    T res[PASSES][8];
+    const int64_t ix = i0 + (wave / WJ) * WTI + 32 * x + lane / PER;
+    if (e.res != nullptr && e.part == nullptr) {            // under way while the slab is written
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) {
+        const int64_t i = ix + p * RPP;
+        const T *rp = (const T *)e.res + i * e.ldres + j;
+        if (FULL || (i < I && n >= 8)) __builtin_memcpy(res[p], rp, sizeof(res[p]));
+        else
+#pragma unroll
+          for (int k = 0; k < 8; ++k) res[p][k] = i < I && k < n ? rp[k] : (T)0.f;
+      }
+    }
+#pragma unroll
+    for (int y = 0; y < G::TJ; ++y)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+          const int row = 8 * (q >> 2) + 4 * (lane >> 5) + (q & 3), c = 32 * y + (lane & 31);
+          slab[row * WTJ + ((((c >> 2) ^ slot_key(row)) << 2) | (c & 3))] = acc[x][y][q];
+        }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+      const int row = p * RPP + lane / PER;
+      const int64_t i = ix + p * RPP;
+      float v[8], r[8];
+      const int s0 = ((c8 >> 2) ^ slot_key(row)) << 2;
+      const f32x4 a = *(LDS_AS f32x4 *)(slab + row * WTJ + s0), b = *(LDS_AS f32x4 *)(slab + row * WTJ + (s0 ^ 4));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) { v[k] = a[k]; v[4 + k] = b[k]; }
+      if (FULL || (i < I && n > 0)) {
+        if (e.part != nullptr) {
+          store8(e.part + ((int64_t)blockIdx.y * I + i) * e.ldp + j, 8, v);   // ldp is a multiple of 8
+        } else {
+          if (e.res != nullptr) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) r[k] = (float)res[p][k];
+          }
+          finish8<T>(e, i, j, n, J, v, r);
+        }
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// One workgroup = one BI x BJ tile of one split.
 template <typename T, bool CA, bool CB, int BI, int BJ, int WI, int WJ, bool DMA>
-__global__ __launch_bounds__(WI *WJ * 64) void k_linear(GemmOperand A, GemmOperand B, Epilogue e, int tiles_i, int tiles_j, int64_t per_split) {
+__global__ __launch_bounds__(WI *WJ * 64, 2) void k_linear(GemmOperand A, GemmOperand B, Epilogue e, int tiles_i, int tiles_j, int64_t per_split) {
   typedef GemmTile<T, CA, CB, BI, BJ, WI, WJ, DMA> G;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -153,48 +258,21 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_linear(GemmOperand A, GemmOpera
   const int64_t i0 = (int64_t)(grp * GRP + in % rows) * BI, j0 = (int64_t)(in / rows) * BJ;
   const int64_t r0 = (int64_t)blockIdx.y * per_split;
   const int64_t r1 = r0 + per_split < A.red ? r0 + per_split : A.red;
-  f32x16 acc[G::TI][G::TJ];
+  f32x16 acc[G::TI][G::TJ];             // starts from the bias of the lane's column (splits: k_linear_join adds it)
 #pragma unroll
-  for (int x = 0; x < G::TI; ++x)
+  for (int y = 0; y < G::TJ; ++y) {
+    const int64_t j = j0 + (wave % WJ) * (BJ / WJ) + 32 * y + (lane & 31);
+    float b = 0.f;
+    if (e.bias != nullptr && e.part == nullptr && j < B.ext) b = e.bias_f32 ? ((const float *)e.bias)[j] : (float)((const T *)e.bias)[j];
 #pragma unroll
-    for (int y = 0; y < G::TJ; ++y)
+    for (int x = 0; x < G::TI; ++x)
 #pragma unroll
-      for (int q = 0; q < 16; ++q) acc[x][y][q] = 0.f;
+      for (int q = 0; q < 16; ++q) acc[x][y][q] = b;
+  }
   G::run(acc, A, B, i0, j0, r0, r1, smem);
 
-  constexpr int WTI = BI / WI, WTJ = BJ / WJ, LDE = WTJ + 8, PER = WTJ / 8, RPP = 64 / PER;   // lanes per row, rows per pass
-  static_assert(WI * WJ * 32 * LDE * 4 <= G::SMEM, "epilogue fits the buffers");
-  LDS_AS float *slab = (LDS_AS float *)(lds_char *)smem + wave * 32 * LDE;
-  const int wi = (wave / WJ) * WTI, wj = (wave % WJ) * WTJ;
-  const int c8 = (lane % PER) * 8;
-  const int64_t j = j0 + wj + c8, J = B.ext;
-  const int n = j >= J ? 0 : (J - j < 8 ? (int)(J - j) : 8);
-  float bias[8];
-  load_bias<T>(e, j, e.part != nullptr ? 0 : n, bias);
-#pragma unroll
-  for (int x = 0; x < G::TI; ++x) {
-#pragma unroll
-    for (int y = 0; y < G::TJ; ++y)
-#pragma unroll
-      for (int q = 0; q < 16; ++q) slab[(8 * (q >> 2) + 4 * (lane >> 5) + (q & 3)) * LDE + 32 * y + (lane & 31)] = acc[x][y][q];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int p = 0; p < 32 / RPP; ++p) {
-      const int row = p * RPP + lane / PER;
-      const int64_t i = i0 + wi + 32 * x + row;
-      float v[8];
-      const f32x4 lo = *(LDS_AS f32x4 *)(slab + row * LDE + c8), hi = *(LDS_AS f32x4 *)(slab + row * LDE + c8 + 4);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) { v[k] = lo[k]; v[4 + k] = hi[k]; }
-      if (i < A.ext && n > 0) {
-        if (e.part != nullptr) store8(e.part + ((int64_t)blockIdx.y * A.ext + i) * e.ldp + j, 8, v);   // ldp is a multiple of 8
-        else finish8<T>(e, i, j, n, J, v, bias);
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-  }
+  if (i0 + BI <= A.ext && j0 + BJ <= B.ext) write_tile<T, BI, BJ, WI, WJ, G, true>(acc, A.ext, B.ext, e, i0, j0, smem, lane, wave);
+  else write_tile<T, BI, BJ, WI, WJ, G, false>(acc, A.ext, B.ext, e, i0, j0, smem, lane, wave);
 }
 
 // sum of the splits in a fixed order, then the epilogue; a thread has eight columns of a row
@@ -214,7 +292,11 @@ __global__ __launch_bounds__(256) void k_linear_join(Epilogue e, int64_t I, int6
     }
     const int n = J - j < 8 ? (int)(J - j) : 8;
     load_bias<T>(e, j, n, b);
-    finish8<T>(e, i, j, n, J, v, b);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] += b[k];
+    float r[8];
+    if (e.res != nullptr) load8((const T *)e.res + i * e.ldres + j, n, r);
+    finish8<T>(e, i, j, n, J, v, r);
   }
 }
 
@@ -224,7 +306,6 @@ template <typename T, int MR, int FPW>
 __global__ __launch_bounds__(256) void k_linear_rows(const T *x, int64_t ldx, const T *w, int M, int64_t K, int64_t N, Epilogue e) {
   constexpr int V = 16 / sizeof(T);
   typedef typename Kept<T>::type Z;
-  constexpr bool FAST = sizeof(T) == 2;
   const int lane = threadIdx.x & 63;
   const int64_t f0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * FPW;
   if (f0 >= N) return;
@@ -267,8 +348,10 @@ __global__ __launch_bounds__(256) void k_linear_rows(const T *x, int64_t ldx, co
         const int64_t j = f0 + f, o = (int64_t)m * N + j;
         float z = s[f][m];
         if (e.bias != nullptr) z += e.bias_f32 ? ((const float *)e.bias)[j] : (float)((const T *)e.bias)[j];
-        if (e.z != nullptr) keep(z, ((Z *)e.z)[o]);
-        float y = act_value<FAST>(z, e.act);
+        if (e.z != nullptr) ((Z *)e.z)[o] = (Z)kept_value(z, e.act);
+        float v[8] = {z, z, z, z, z, z, z, z};
+        act8<sizeof(T) == 2>(v, e.act);
+        float y = v[0];
         if (e.res != nullptr) y += (float)((const T *)e.res)[(int64_t)m * e.ldres + j];
         ((T *)e.out)[o] = (T)y;
       }
@@ -280,7 +363,6 @@ template <typename T>
 __global__ __launch_bounds__(256) void k_linear_dz(const T *dy, const void *zv, T *dz, float *part, int64_t M, int64_t N, int64_t rows, int act,
                                                    void *db, int db_f32) {
   typedef typename Kept<T>::type Z;
-  constexpr bool FAST = sizeof(T) == 2;
   __shared__ float red[4][512];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t j = (int64_t)blockIdx.x * 512 + lane * 8;
@@ -296,8 +378,7 @@ __global__ __launch_bounds__(256) void k_linear_dz(const T *dy, const void *zv, 
       if (dz != nullptr) {
         float z[8];
         load8((const Z *)zv + m * N + j, n, z);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) g[k] *= act_slope<FAST>(z[k], act);
+        slope8<sizeof(T) == 2>(g, z, act);
         store8(dz + m * N + j, n, g);
       }
 #pragma unroll
@@ -317,22 +398,25 @@ __global__ __launch_bounds__(256) void k_linear_dz(const T *dy, const void *zv, 
   }
 }
 
-// out[col] = sum over P partial rows, in a fixed order: 64 columns per workgroup, four waves over the partials
+// out[col] = sum over P partial rows, in a fixed order: 32 columns per workgroup, 32 groups of lanes over the partials
 template <typename T>
-__global__ __launch_bounds__(256) void k_column_join(const float *part, int P, int64_t N, void *out, int out_f32) {
-  __shared__ float red[4][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t col = (int64_t)blockIdx.x * 64 + lane;
+__global__ __launch_bounds__(1024) void k_column_join(const float *part, int P, int64_t N, void *out, int out_f32) {
+  __shared__ float red[32][33];
+  const int c = threadIdx.x & 31, grp = threadIdx.x >> 5;
+  const int64_t col = (int64_t)blockIdx.x * 32 + c;
   float s = 0.f;
-  if (col < N)
-    for (int p = wave; p < P; p += 4) s += part[(int64_t)p * N + col];
-  red[wave][lane] = s;
-  __syncthreads();
-  if (wave == 0 && col < N) {
-    const float t = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
-    if (out_f32) ((float *)out)[col] = t;
-    else ((T *)out)[col] = (T)t;
+  if (col < N) {
+#pragma unroll 8
+    for (int p = grp; p < P; p += 32) s += part[(int64_t)p * N + col];
   }
+  red[grp][c] = s;
+  __syncthreads();
+  if (threadIdx.x >= 32 || col >= N) return;
+  float t = 0.f;
+#pragma unroll
+  for (int g = 0; g < 32; ++g) t += red[g][c];
+  if (out_f32) ((float *)out)[col] = t;
+  else ((T *)out)[col] = (T)t;
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
@@ -342,7 +426,7 @@ inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t align256(int64_t b) { return (b + 255) & ~(int64_t)255; }
 inline int elem_size(int dt) { return dt == CINEMA_DT_F32 ? 4 : 2; }
 
-struct Plan { int tile; int splits; int64_t per_split, ti, tj, ldp, part_bytes; };   // tile: 64 or 128
+struct Plan { int tile; int splits; int64_t per_split, ti, tj, ldp, part_bytes; };   // tile: 64, 128 or 256
 
 Plan plan_product(int64_t I, int64_t J, int64_t R, int dt) {
   Plan p;
@@ -363,20 +447,27 @@ Plan plan_product(int64_t I, int64_t J, int64_t R, int dt) {
   return p;
 }
 
-template <typename T, bool CA, bool CB, int BT, bool DMA>
+template <typename T, bool CA, bool CB, int BI, int BJ, int WI, int WJ, bool DMA>
 int launch_tile(const GemmOperand &A, const GemmOperand &B, const Epilogue &e, const Plan &p, hipStream_t st) {
-  typedef GemmTile<T, CA, CB, BT, BT, 2, 2, DMA> G;
-  auto fn = k_linear<T, CA, CB, BT, BT, 2, 2, DMA>;
+  typedef GemmTile<T, CA, CB, BI, BJ, WI, WJ, DMA> G;
+  auto fn = k_linear<T, CA, CB, BI, BJ, WI, WJ, DMA>;
   CINEMA_SMEM_ATTR(fn, G::SMEM);
-  hipLaunchKernelGGL(fn, dim3((unsigned)(p.ti * p.tj), (unsigned)p.splits), dim3(256), G::SMEM, st, A, B, e, (int)p.ti, (int)p.tj, p.per_split);
+  hipLaunchKernelGGL(fn, dim3((unsigned)(p.ti * p.tj), (unsigned)p.splits), dim3(WI * WJ * 64), G::SMEM, st, A, B, e, (int)p.ti, (int)p.tj, p.per_split);
   CINEMA_CHECK_HIP(hipGetLastError());
   return 0;
+}
+
+// 256 x 256 tiles (one workgroup of eight waves on a compute unit) ask the L2 for half the bytes of 128 x 128 tiles (two
+// workgroups of four waves): taken where they do not leave more of the last round empty
+bool large_tiles(int64_t I, int64_t J) {
+  const int64_t cu = cinema_cu_count();
+  return up(up(I, 256) * up(J, 256), cu) * 4 <= up(up(I, 128) * up(J, 128), 2 * cu) * 2;
 }
 
 template <typename T>
 bool whole_chunks(const GemmOperand &o, bool col) {
   constexpr int V = 16 / sizeof(T);
-  return ((uintptr_t)o.p & 15) == 0 && o.ld % V == 0 && (col ? o.ext : o.red) % V == 0;
+  return ((uintptr_t)o.p & 15) == 0 && o.ld % V == 0 && (col ? o.ext : o.red) % V == 0 && o.ld < (1 << 20);   // 256 rows below 2 GB
 }
 
 // C = A B^T with the epilogue; part = workspace of plan.part_bytes
@@ -387,8 +478,16 @@ int product(const GemmOperand &A, const GemmOperand &B, Epilogue e, int dt, void
   e.part = p.splits > 1 ? (float *)part : nullptr;
   const bool dma = whole_chunks<T>(A, CA) && whole_chunks<T>(B, CB);
   int rc;
-  if (p.tile == 128) rc = dma ? launch_tile<T, CA, CB, 128, true>(A, B, e, p, st) : launch_tile<T, CA, CB, 128, false>(A, B, e, p, st);
-  else rc = dma ? launch_tile<T, CA, CB, 64, true>(A, B, e, p, st) : launch_tile<T, CA, CB, 64, false>(A, B, e, p, st);
+  if constexpr (sizeof(T) == 2) {
+    if (dma && p.tile == 128 && p.splits == 1 && large_tiles(A.ext, B.ext)) {
+      Plan q = p;
+      q.ti = up(A.ext, 256);
+      q.tj = up(B.ext, 256);
+      return launch_tile<T, CA, CB, 256, 256, 2, 4, true>(A, B, e, q, st);
+    }
+  }
+  if (p.tile == 128) rc = dma ? launch_tile<T, CA, CB, 128, 128, 2, 2, true>(A, B, e, p, st) : launch_tile<T, CA, CB, 128, 128, 2, 2, false>(A, B, e, p, st);
+  else rc = dma ? launch_tile<T, CA, CB, 64, 64, 2, 2, true>(A, B, e, p, st) : launch_tile<T, CA, CB, 64, 64, 2, 2, false>(A, B, e, p, st);
   if (rc != 0 || p.splits == 1) return rc;
   const int64_t groups = A.ext * (p.ldp >> 3);
   hipLaunchKernelGGL(k_linear_join<T>, dim3((unsigned)std::min<int64_t>(up(groups, 256), 4096)), dim3(256), 0, st, e, A.ext, B.ext, p.splits);
@@ -408,9 +507,9 @@ int check_sizes(const char *who, int64_t M, int64_t K, int64_t N, int dt) {
   return 0;
 }
 
-// rows of dz per workgroup of k_linear_dz: enough workgroups to fill the chip, sums of at most 64 partials where that allows it
+// rows of dz per workgroup of k_linear_dz: enough workgroups to fill the chip, two for a compute unit
 int64_t dz_rows(int64_t M, int64_t N) {
-  const int64_t bx = up(N, 512), by = std::max<int64_t>(1, std::min<int64_t>(up(M, 16), up(4 * cinema_cu_count(), bx)));
+  const int64_t bx = up(N, 512), by = std::max<int64_t>(1, std::min<int64_t>(up(M, 16), up(2 * cinema_cu_count(), bx)));
   return up(M, by);
 }
 
@@ -458,7 +557,7 @@ int backward_t(const void *dy, const void *z, const void *x, int64_t ldx, const 
     CINEMA_CHECK_HIP(hipGetLastError());
     if (out != nullptr) dz = out;
     if (db != nullptr && P > 1) {
-      hipLaunchKernelGGL(k_column_join<T>, dim3((unsigned)up(N, 64)), dim3(256), 0, st, part, (int)P, N, db, db_f32);
+      hipLaunchKernelGGL(k_column_join<T>, dim3((unsigned)up(N, 32)), dim3(1024), 0, st, part, (int)P, N, db, db_f32);
       CINEMA_CHECK_HIP(hipGetLastError());
     }
   }

@@ -2,12 +2,13 @@
 //
 // Each operand lies in memory in one of two ways: ROW = [i][r], the reduction contiguous (x and W of x W^T), or COL =
 // [r][i], the reduction across rows (W in dz W, both operands of dz^T x).  A 16-byte piece ("chunk") is 8 bf16 / fp16 or
-// 4 fp32 values; a reduction tile is 128 bytes of a ROW operand (64 or 32 values of r).
+// 4 fp32 values; a reduction tile is 128 bytes of a ROW operand (64 or 32 values of r).  64-byte tiles in a ring of four lost: a copy
+// then asks the L2 for 64 bytes at a time, and 128 x 128 tiles on 32768 x 4096 x 4096 ran at 890 instead of 1190 TFLOP/s.
 //
 // LDS images hold the chunks without padding, so that the copy global -> LDS can go past the registers
 // (global_load_lds_dwordx4: a wave writes 1024 consecutive bytes, the lanes choose what they fetch):
-//   ROW: rows of 128 bytes; chunk c of row i sits in slot c ^ (i & 7), so the 32 rows of a fragment spread over all banks.
-//   COL, 16-bit: rows of the tile's width; chunk c of row r sits in slot c ^ col_key(r), ds_read_b64_tr_b16 transposes
+//   ROW: rows of 128 bytes; chunk c of row i sits in slot c ^ key(i), so the 32 rows of a fragment spread over all banks.
+//   COL, 16-bit: rows of the tile's width; chunk c of row r sits in slot c ^ key(r), ds_read_b64_tr_b16 transposes
 //        4 x 16 values per 16 lanes on the way out.     COL, fp32: rows as they are, one 4-byte read per value.
 // The matrix instruction is 32x32x16 (16-bit) or four 32x32x2 (fp32): lane l feeds row l & 31 and the chunk 2 * kk + (l >> 5),
 // in both operands alike, so any order of r inside a tile gives the same product.  Result register q of lane l is
@@ -47,12 +48,17 @@ template <> struct Mma<float> {
 // 16 zero bytes that lanes outside the reduction fetch instead
 __device__ const u32x4 g_zero_chunk = {0u, 0u, 0u, 0u};
 
-// 16 bytes per lane from `src` to LDS byte address `lds` (wave-uniform) + 16 * lane.  No compiler-visible load: the caller
-// waits with vmcnt.  m0 carries the LDS address of the instruction and is put back.
+// 16 bytes per lane from `src`, or from `base` (wave-uniform) + off bytes, to LDS byte address `lds` (wave-uniform) + 16 * lane.
+// No compiler-visible load: the caller waits with vmcnt.  m0 carries the LDS address of the instruction and is put back.
 __device__ __forceinline__ void copy_to_lds(const void *src, unsigned lds) {
   unsigned keep;
   asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
                : "=&s"(keep) : "v"(src), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void copy_to_lds(const void *base, unsigned off, unsigned lds) {
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "v"(off), "s"(base), "s"(lds) : "memory");
 }
 
 template <typename T>
@@ -71,84 +77,102 @@ __device__ __forceinline__ u32x4 load_chunk(const T *p, int n) {   // n valid va
 }
 
 // One operand of a workgroup's tile: NROW rows of i, copied by NW waves.  DMA: chunks are whole and 16-byte aligned
-// (ld, ext of COL, red of ROW are multiples of a chunk); otherwise they pass through registers, value by value at the edge.
+// (ld, ext of COL, red of ROW are multiples of a chunk) and go to LDS directly; otherwise they pass through registers, value
+// by value where a chunk is cut by an end.
 template <typename T, bool COL, int NROW, int NW, bool DMA>
 struct TileCopy {
   static constexpr int V = 16 / sizeof(T);
   static constexpr int RT = 128 / sizeof(T);                          // values of r in a tile
   static constexpr int CPR = COL ? NROW / V : 8;                      // chunks in an LDS row
-  static constexpr int ROWS = COL ? RT : NROW;                        // LDS rows
   static constexpr int BYTES = NROW * 128;
   static constexpr int NC = BYTES / 1024 / NW;                        // 1024-byte pieces per wave
-  static_assert(NC >= 1, "tile too small for this many waves");
-  const T *src[NC];
-  int chunk0[NC];           // ROW: first r of the chunk inside a tile; COL: r of the chunk inside a tile
-  int nvalid[NC];           // COL: valid values of i in the chunk (without DMA)
+  static_assert(NC >= 1 && BYTES % (1024 * NW) == 0, "tile too small for this many waves");
+  const T *base;            // first value of the workgroup's rows (ROW) or columns (COL) in the next tile; wave-uniform
+  int64_t off[DMA ? 1 : NC];
+  unsigned off32[DMA ? NC : 1];   // bytes from base; the host takes DMA only where a tile spans less than 2 GB
+  int chunk0[NC];           // r of the chunk's first value inside a tile
+  int nvalid[DMA ? 1 : NC]; // COL: values of i in the chunk that exist
   u32x4 st[DMA ? 1 : NC];
   int64_t step;             // elements from tile to tile
-  int64_t left;             // values of r from the current tile on
+  int64_t left;             // values of r from the next tile on
+  bool whole;               // COL: no chunk of the workgroup is cut by the end of i
 
   __device__ static __forceinline__ int key(int row) {
-    if (!COL) return row & 7;
-    if (sizeof(T) == 4) return 0;
-    if (NROW >= 128) return ((row & 3) << 1) | (((row >> 3) & 1) << 3);
-    return (row & 3) << 1;
+    // 64 banks: 16 lanes of a 16-byte read, 32 lanes of an 8-byte read and 64 lanes of a 4-byte read share a cycle
+    if (!COL) return (row >> 1) & 7;
+    if (sizeof(T) == 4) return ((row >> 2) & 1) << 3;
+    return NROW >= 128 ? (row & 3) << 2 : (row & 2) << 1;
   }
   __device__ __forceinline__ void init(const GemmOperand &o, int64_t i0, int64_t r0, int64_t r1, int wave, int lane) {
     left = r1 - r0;
     step = COL ? (int64_t)RT * o.ld : RT;
+    whole = !COL || i0 + NROW <= o.ext;
+    base = (const T *)o.p + (COL ? r0 * o.ld + i0 : i0 * o.ld + r0);
 #pragma unroll
     for (int q = 0; q < NC; ++q) {
       const int c = ((wave * NC + q) * 64 + lane);                    // chunk number in the image
       const int row = c / CPR, ch = (c % CPR) ^ key(row);
+      int64_t at;
       if (COL) {
-        const int64_t i = i0 + ch * V;
-        const bool in = i < o.ext;
-        src[q] = (const T *)o.p + (r0 + row) * o.ld + (in ? i : 0);
+        const int64_t n = o.ext - (i0 + ch * V);
+        at = (int64_t)row * o.ld + (n > 0 ? ch * V : 0);
         chunk0[q] = row;
-        const int64_t n = o.ext - i;
-        nvalid[q] = in ? (n < V ? (int)n : V) : 0;
+        if (!DMA) nvalid[q] = n <= 0 ? 0 : (n < V ? (int)n : V);
       } else {
-        int64_t i = i0 + row;
-        if (i >= o.ext) i = o.ext - 1;                                // rows past the end repeat the last: never stored
-        src[q] = (const T *)o.p + i * o.ld + r0 + ch * V;
+        const int64_t last = o.ext - 1 - i0;                          // rows past the end repeat the last: never stored
+        at = (row < last ? row : last) * o.ld + ch * V;
         chunk0[q] = ch * V;
-        nvalid[q] = V;
+        if (!DMA) nvalid[q] = V;
       }
+      if (DMA) off32[q] = (unsigned)at * (unsigned)sizeof(T);
+      else off[q] = at;
     }
   }
-  __device__ __forceinline__ void load(unsigned lds, int wave) {
+  // DMA: piece q of the next tile.  WHOLE: the tile is whole in r; else what is past the end comes as zeros.
+  template <bool WHOLE>
+  __device__ __forceinline__ void copy(int q, unsigned lds, int wave) const {
+    const unsigned to = lds + (unsigned)(wave * NC + q) * 1024u;
+    if (WHOLE) copy_to_lds(base, off32[q], to);
+    else copy_to_lds(left > chunk0[q] ? (const void *)((const char *)base + off32[q]) : (const void *)&g_zero_chunk, to);
+  }
+  __device__ __forceinline__ void advance() {
+    base += step;
+    left -= RT;
+  }
+  // through registers
+  __device__ __forceinline__ void load() {
+    if (left >= RT && whole) {                                        // uniform
 #pragma unroll
-    for (int q = 0; q < NC; ++q) {
-      const int64_t n = left - chunk0[q];
-      if (DMA) {
-        copy_to_lds(n > 0 ? (const void *)src[q] : (const void *)&g_zero_chunk, lds + (unsigned)(wave * NC + q) * 1024u);
-      } else {
-        const int m = n <= 0 ? 0 : (COL ? nvalid[q] : (n < V ? (int)n : V));
-        st[q] = load_chunk(src[q], m);
+      for (int q = 0; q < NC; ++q) __builtin_memcpy(&st[DMA ? 0 : q], base + off[DMA ? 0 : q], 16);
+    } else {
+#pragma unroll
+      for (int q = 0; q < NC; ++q) {
+        const int64_t n = left - chunk0[q];
+        st[DMA ? 0 : q] = load_chunk(base + off[DMA ? 0 : q], n <= 0 ? 0 : (COL ? nvalid[DMA ? 0 : q] : (n < V ? (int)n : V)));
       }
-      src[q] += step;
     }
+    base += step;
     left -= RT;
   }
   __device__ __forceinline__ void store(lds_char *tile, int wave, int lane) {
-    if (!DMA) {
 #pragma unroll
-      for (int q = 0; q < NC; ++q) *(LDS_AS u32x4 *)(tile + ((wave * NC + q) * 64 + lane) * 16) = st[q];
-    }
+    for (int q = 0; q < NC; ++q) *(LDS_AS u32x4 *)(tile + ((wave * NC + q) * 64 + lane) * 16) = st[DMA ? 0 : q];
   }
   // fragment of rows i..i+31 of the tile, chunk pair kk
   __device__ static __forceinline__ typename Mma<T>::frag frag(const lds_char *tile, int i, int kk, int lane) {
     typedef typename Mma<T>::frag F;
     const int h = lane >> 5;
-    if (!COL) {
+    if constexpr (!COL) {
       const int row = i + (lane & 31), ch = 2 * kk + h;
       return *(const LDS_AS F *)(tile + row * 128 + ((ch ^ key(row)) << 4));
     } else if constexpr (sizeof(T) == 4) {
       F f;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        f[e] = *(const LDS_AS float *)(tile + (((2 * kk + h) * 4 + e) * NROW + i + (lane & 31)) * 4);
+      {
+        const int r = (2 * kk + h) * 4 + e, col = i + (lane & 31);
+        f[e] = *(const LDS_AS float *)(tile + r * (CPR * 16) + (((col >> 2) ^ key(r)) << 4) + (col & 3) * 4);
+      }
       return f;
     } else {
       // 16 lanes: 16 columns, 4 rows per read; lane 4q + p addresses row q, columns 4p .. 4p + 3
@@ -164,16 +188,84 @@ struct TileCopy {
   }
 };
 
-// Tile of BI x BJ results on WI x WJ waves; acc[a][b] are the wave's 32 x 32 blocks.  Two LDS buffers: the copy of tile t + 1
-// runs while tile t is multiplied; one barrier per tile.
+__device__ __forceinline__ void wait_copies() {      // this wave's copies have arrived
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+// barrier alone, without waiting for this wave's own loads and stores
+__device__ __forceinline__ void bare_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Tile of BI x BJ results on WI x WJ waves; acc[a][b] are the wave's 32 x 32 blocks.  Two LDS buffers, one barrier per tile of
+// r: it publishes the copies of tile t and frees the other buffer for those of tile t + 1, which run while tile t is
+// multiplied.  Fragments are read one step (two chunks of r) ahead of the matrix instructions.
 template <typename T, bool CA, bool CB, int BI, int BJ, int WI, int WJ, bool DMA>
 struct GemmTile {
   static constexpr int NW = WI * WJ, TI = BI / WI / 32, TJ = BJ / WJ / 32;
   typedef TileCopy<T, CA, BI, NW, DMA> LA;
   typedef TileCopy<T, CB, BJ, NW, DMA> LB;
+  typedef typename Mma<T>::frag F;
   static constexpr int STAGE = LA::BYTES + LB::BYTES;
   static constexpr int SMEM = 2 * STAGE;
   static constexpr int RT = LA::RT;
+
+  struct Frags { F a[TI], b[TJ]; };
+  __device__ static __forceinline__ void read_one(Frags &f, int n, const lds_char *stage, int kk, int wi, int wj, int lane) {
+    if (n < TJ) f.b[n] = LB::frag(stage + LA::BYTES, wj + 32 * n, kk, lane);      // the first product needs b[0] and a[0]
+    else f.a[n - TJ] = LA::frag(stage, wi + 32 * (n - TJ), kk, lane);
+  }
+  __device__ static __forceinline__ void read(Frags &f, const lds_char *stage, int kk, int wi, int wj, int lane) {
+#pragma unroll
+    for (int n = 0; n < TI + TJ; ++n) read_one(f, n, stage, kk, wi, wj, lane);
+  }
+  __device__ static __forceinline__ void multiply(f32x16 (&acc)[TI][TJ], const Frags &f) {
+#pragma unroll
+    for (int x = 0; x < TI; ++x)
+#pragma unroll
+      for (int y = 0; y < TJ; ++y) acc[x][y] = Mma<T>::mma(f.a[x], f.b[y], acc[x][y]);
+  }
+  // the products of `f`, the reads of the next fragments and `copies` copies (issue(c) makes one) in between: the matrix unit
+  // starts at once instead of behind the queue of all waves' reads and copies
+  template <int COPIES, typename ISSUE>
+  __device__ static __forceinline__ void multiply_and_read(f32x16 (&acc)[TI][TJ], const Frags &f, Frags &next, const lds_char *stage, int kk,
+                                                           int wi, int wj, int lane, ISSUE issue) {
+    constexpr int N = TI * TJ, R = TI + TJ;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      acc[n / TJ][n % TJ] = Mma<T>::mma(f.a[n / TJ], f.b[n % TJ], acc[n / TJ][n % TJ]);
+#pragma unroll
+      for (int r = n * R / (N > R ? R : N); r < (n + 1) * R / (N > R ? R : N) && r < R; ++r) read_one(next, r, stage, kk, wi, wj, lane);
+#pragma unroll
+      for (int c = n * COPIES / N; c < (n + 1) * COPIES / N; ++c) issue(c);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  // tile t is multiplied, tile t + 1 copied.  NEXT: 0 there is none, 1 it is whole in r, 2 it may be cut
+  template <int NEXT>
+  __device__ static __forceinline__ void tile(f32x16 (&acc)[TI][TJ], LA &la, LB &lb, int t, lds_char *base, unsigned lds0, int wi, int wj,
+                                              int lane, int wave) {
+    constexpr int C = NEXT ? LA::NC + LB::NC : 0, H = (C + 1) / 2;
+    const lds_char *cur = base + (t & 1) * STAGE;
+    const unsigned to = lds0 + ((t & 1) ^ 1) * STAGE;
+    auto issue = [&](int c) {
+      if (c < LA::NC) la.template copy<NEXT == 1>(c, to, wave);
+      else lb.template copy<NEXT == 1>(c - LA::NC, to + LA::BYTES, wave);
+    };
+    wait_copies();
+    bare_barrier();
+    Frags f0, f1;
+    read(f0, cur, 0, wi, wj, lane);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply_and_read<H>(acc, f0, f1, cur, 1, wi, wj, lane, issue);
+    multiply_and_read<C - H>(acc, f1, f0, cur, 2, wi, wj, lane, [&](int c) { issue(c + H); });
+    la.advance();
+    lb.advance();
+    multiply_and_read<0>(acc, f0, f1, cur, 3, wi, wj, lane, [](int) {});
+    multiply(acc, f1);
+    __builtin_amdgcn_sched_barrier(0);
+  }
 
   __device__ static __forceinline__ void run(f32x16 (&acc)[TI][TJ], const GemmOperand &A, const GemmOperand &B, int64_t i0,
                                              int64_t j0, int64_t r0, int64_t r1, char *smem) {
@@ -187,36 +279,42 @@ struct GemmTile {
     lb.init(B, j0, r0, r1, wave, lane);
     const int nt = (int)((r1 - r0 + RT - 1) / RT);
     if (nt <= 0) return;
-    la.load(lds0, wave);
-    lb.load(lds0 + LA::BYTES, wave);
-    la.store(base, wave, lane);
-    lb.store(base + LA::BYTES, wave, lane);
-    for (int t = 0; t < nt; ++t) {
-      const int cur = t & 1, nxt = cur ^ 1;
-      if (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();        // tile t is there for every wave, and every wave is done with tile t - 1
-      if (t + 1 < nt) {
-        la.load(lds0 + nxt * STAGE, wave);
-        lb.load(lds0 + nxt * STAGE + LA::BYTES, wave);
-      }
-      const lds_char *ta = base + cur * STAGE, *tb = ta + LA::BYTES;
+    if constexpr (DMA) {
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        typename Mma<T>::frag a[TI], b[TJ];
+      for (int q = 0; q < LA::NC; ++q) la.template copy<false>(q, lds0, wave);
 #pragma unroll
-        for (int x = 0; x < TI; ++x) a[x] = LA::frag(ta, wi + 32 * x, kk, lane);
+      for (int q = 0; q < LB::NC; ++q) lb.template copy<false>(q, lds0 + LA::BYTES, wave);
+      la.advance();
+      lb.advance();
+      int t = 0;
+      const int whole = (int)((r1 - r0) / RT) - 1;          // tiles whose successor is whole
+      for (; t < whole; ++t) tile<1>(acc, la, lb, t, base, lds0, wi, wj, lane, wave);
+      for (; t < nt - 1; ++t) tile<2>(acc, la, lb, t, base, lds0, wi, wj, lane, wave);
+      tile<0>(acc, la, lb, t, base, lds0, wi, wj, lane, wave);
+    } else {
+      la.load();
+      lb.load();
+      la.store(base, wave, lane);
+      lb.store(base + LA::BYTES, wave, lane);
+      for (int t = 0; t < nt; ++t) {
+        lds_char *cur = base + (t & 1) * STAGE, *nxt = base + ((t & 1) ^ 1) * STAGE;
+        __syncthreads();        // tile t is there for every wave, and every wave is done with tile t - 1
+        if (t + 1 < nt) {
+          la.load();
+          lb.load();
+        }
 #pragma unroll
-        for (int y = 0; y < TJ; ++y) b[y] = LB::frag(tb, wj + 32 * y, kk, lane);
-#pragma unroll
-        for (int x = 0; x < TI; ++x)
-#pragma unroll
-          for (int y = 0; y < TJ; ++y) acc[x][y] = Mma<T>::mma(a[x], b[y], acc[x][y]);
-      }
-      if (t + 1 < nt) {
-        la.store(base + nxt * STAGE, wave, lane);
-        lb.store(base + nxt * STAGE + LA::BYTES, wave, lane);
+        for (int kk = 0; kk < 4; ++kk) {
+          Frags f;
+          read(f, cur, kk, wi, wj, lane);
+          multiply(acc, f);
+        }
+        if (t + 1 < nt) {
+          la.store(nxt, wave, lane);
+          lb.store(nxt + LA::BYTES, wave, lane);
+        }
       }
     }
-    __syncthreads();          // the caller's epilogue reuses the buffers
+    __syncthreads();            // the caller's epilogue reuses the buffers
   }
 };
