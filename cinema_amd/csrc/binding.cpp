@@ -133,8 +133,9 @@ struct LinearActBackward : public Node {
     if (m == 0) return got;
     const Tensor xs = x.unpack(), ws = w.unpack(), zs = z.unpack();
     const int dt = dtype_of(g.scalar_type());
-    const Tensor work = workspace(api.linear_work_bytes(m, k, n, dt, 1), "cinema_linear_work_bytes", g);
-    check(api.linear_backward(data(g), data(zs), need_w ? data(xs) : nullptr, ldx, need_x ? data(ws) : nullptr, m, k, n, act, dt,
+    const void *xp = need_w ? data(xs) : nullptr, *wp = need_x ? data(ws) : nullptr;
+    const Tensor work = workspace(api.linear_work_bytes(xp, ldx, wp, m, k, n, dt, 1), "cinema_linear_work_bytes", g);
+    check(api.linear_backward(data(g), data(zs), xp, ldx, wp, m, k, n, act, dt,
                               bias_type == at::kFloat, out(got[0]), out(got[1]), out(got[2]), out(work), stream_of(g)),
           "cinema_linear_backward");
     return got;
@@ -192,7 +193,7 @@ Tensor linear_act(Tensor x, Tensor w, const MaybeTensor &bias, const MaybeTensor
     if (r.defined()) rr = rows_of(r, n);
     if (m > 0) {
       const int dt = dtype_of(x.scalar_type());
-      const Tensor work = workspace(api.linear_work_bytes(m, k, n, dt, 0), "cinema_linear_work_bytes", x);
+      const Tensor work = workspace(api.linear_work_bytes(data(xr.t), xr.ld, data(wc), m, k, n, dt, 0), "cinema_linear_work_bytes", x);
       check(api.linear_forward(data(xr.t), xr.ld, data(wc), data(bc), bc.defined() && bc.scalar_type() == at::kFloat, data(rr.t), rr.ld, m, k, n,
                                act, dt, out(z), out(y), out(work), stream_of(x)),
             "cinema_linear_forward");

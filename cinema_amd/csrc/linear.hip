@@ -114,6 +114,21 @@ template <typename T> struct Kept { typedef f16_t type; };
 template <> struct Kept<float> { typedef float type; };
 __device__ __forceinline__ float kept_value(float z, int act) { return act == ACT_RELU ? (z <= 0.f ? 0.f : (z > 0.f ? 1.f : z)) : z; }
 
+template <typename T>
+__device__ __forceinline__ u32x4 load_chunk(const T *p, int n) {   // n valid values, the others read as zero
+  constexpr int V = 16 / sizeof(T);
+  u32x4 r = {0u, 0u, 0u, 0u};
+  if (n >= V) {
+    __builtin_memcpy(&r, p, 16);        // 2- or 4-byte aligned: one dwordx4 in the target's unaligned mode
+  } else if (n > 0) {
+    T e[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) e[k] = k < n ? p[k] : (T)0.f;
+    __builtin_memcpy(&r, e, 16);
+  }
+  return r;
+}
+
 template <typename S>
 __device__ __forceinline__ void load8(const S *p, int n, float (&v)[8]) {
   if (n >= 8) {
@@ -245,9 +260,9 @@ __device__ __forceinline__ void write_tile(const f32x16 (&acc)[G::TI][G::TJ], in
 }
 
 // One workgroup = one BI x BJ tile of one split.
-template <typename T, bool CA, bool CB, int BI, int BJ, int WI, int WJ, bool DMA>
+template <typename T, bool CA, bool CB, int BI, int BJ, int WI, int WJ>
 __global__ __launch_bounds__(WI *WJ * 64, 2) void k_linear(GemmOperand A, GemmOperand B, Epilogue e, int tiles_i, int tiles_j, int64_t per_split) {
-  typedef GemmTile<T, CA, CB, BI, BJ, WI, WJ, DMA> G;
+  typedef GemmTile<T, CA, CB, BI, BJ, WI, WJ> G;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // tiles that share rows of A follow each other on one XCD (its L2 then holds them): blocks of 8 row tiles, row tile fastest
@@ -358,10 +373,11 @@ __global__ __launch_bounds__(256) void k_linear_rows(const T *x, int64_t ldx, co
 }
 
 // dz = dy * act'(z) and the column sums of dz over the block's rows.  A workgroup takes 512 columns (64 lanes x 8) and `rows`
-// rows, its four waves every fourth row; sums of the waves meet in LDS.  dz == null: only the sums (no activation).
+// rows, its four waves every fourth row; sums of the waves meet in LDS.  dz has rows of ldz values, zeros behind the N'th (the
+// products read whole chunks).  dz == null: only the sums.
 template <typename T>
-__global__ __launch_bounds__(256) void k_linear_dz(const T *dy, const void *zv, T *dz, float *part, int64_t M, int64_t N, int64_t rows, int act,
-                                                   void *db, int db_f32) {
+__global__ __launch_bounds__(256) void k_linear_dz(const T *dy, const void *zv, T *dz, int64_t ldz, float *part, int64_t M, int64_t N, int64_t rows,
+                                                   int act, void *db, int db_f32) {
   typedef typename Kept<T>::type Z;
   __shared__ float red[4][512];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -376,10 +392,14 @@ __global__ __launch_bounds__(256) void k_linear_dz(const T *dy, const void *zv, 
       float g[8];
       load8(dy + m * N + j, n, g);
       if (dz != nullptr) {
-        float z[8];
-        load8((const Z *)zv + m * N + j, n, z);
-        slope8<sizeof(T) == 2>(g, z, act);
-        store8(dz + m * N + j, n, g);
+        if (act != ACT_NONE) {
+          float z[8];
+          load8((const Z *)zv + m * N + j, n, z);
+          slope8<sizeof(T) == 2>(g, z, act);
+          if (n < 8)
+            for (int k = n; k < 8; ++k) g[k] = 0.f;                   // 0 * slope of nothing
+        }
+        store8(dz + m * ldz + j, ldz - j < 8 ? (int)(ldz - j) : 8, g);
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) sum[k] += k < n ? g[k] : 0.f;
@@ -395,6 +415,22 @@ __global__ __launch_bounds__(256) void k_linear_dz(const T *dy, const void *zv, 
     if (gridDim.y > 1) part[(int64_t)blockIdx.y * N + col] = t;
     else if (db_f32) ((float *)db)[col] = t;
     else ((T *)db)[col] = (T)t;
+  }
+}
+
+// rows [R][ld] of C values -> [R][ldo], ldo the next multiple of a chunk, zeros behind; a thread moves a chunk.  Two at once.
+struct Pack { const void *src; void *dst; int64_t rows, cols, ld, ldo; };
+template <typename T>
+__global__ __launch_bounds__(256) void k_linear_pack(Pack a, Pack b) {
+  const Pack p = blockIdx.y == 0 ? a : b;
+  constexpr int V = 16 / sizeof(T);
+  const unsigned per = (unsigned)(p.ldo / V);
+  const int64_t total = p.rows * per;
+  for (int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x; g < total; g += (int64_t)gridDim.x * 256) {
+    const int64_t row = total <= 0xffffffffll ? (int64_t)((unsigned)g / per) : g / per;
+    const int64_t c = (g - row * per) * V;
+    const u32x4 v = load_chunk((const T *)p.src + row * p.ld + c, p.cols - c < V ? (int)(p.cols - c) : V);
+    *(u32x4 *)((T *)p.dst + row * p.ldo + c) = v;
   }
 }
 
@@ -428,46 +464,89 @@ inline int elem_size(int dt) { return dt == CINEMA_DT_F32 ? 4 : 2; }
 
 struct Plan { int tile; int splits; int64_t per_split, ti, tj, ldp, part_bytes; };   // tile: 64, 128 or 256
 
+// Tile and number of splits by an estimate of the time in microseconds.  A compute unit takes `step` for 128 bytes of r of a
+// tile and `fixed` for a tile's start and epilogue, whether its tiles run side by side or one after the other; both were fitted
+// to 25000 x 512, 8192 x 1280, 2048 x 2048 and 32768 x 4096 outputs over r = 64 .. 4096, and tell the fastest tile there in all
+// but near ties.  What a step costs is the L2's rate: 16, 32, 64 KB of operands at 64 to 80 GB/s and compute unit (16-bit); fp32
+// is bound by the matrix unit.  A split writes and reads its fp32 sums once more.
+struct TileCost { int tile; double step, fixed; };
+constexpr TileCost COST_16[] = {{64, 0.2, 0.8}, {128, 0.4, 2.6}, {256, 1.2, 13.}};
+constexpr TileCost COST_32[] = {{64, 0.5, 1.0}, {128, 1.8, 4.5}};
+
 Plan plan_product(int64_t I, int64_t J, int64_t R, int dt) {
-  Plan p;
-  const int cu = cinema_cu_count();
-  const int64_t rt = 128 / elem_size(dt);
-  p.tile = up(I, 128) * up(J, 128) * 2 >= cu && I > 64 && J > 64 ? 128 : 64;
-  // many small problems: weight gradients reduce over all rows and have few output tiles
-  if (p.tile == 64 && I >= 128 && J >= 128 && R >= 2048) p.tile = 128;
-  p.ti = up(I, p.tile);
-  p.tj = up(J, p.tile);
-  const int64_t nt = up(R, rt);
-  // a split costs a write and a read of its fp32 tile: at least 8 reduction tiles each, and no more than fill the chip twice
-  int64_t s = std::max<int64_t>(1, std::min<int64_t>(2 * cu / (p.ti * p.tj), nt / 8));
-  p.per_split = up(nt, s) * rt;
-  p.splits = (int)up(R, p.per_split);
-  p.ldp = (J + 7) & ~(int64_t)7;
-  p.part_bytes = p.splits > 1 ? align256((int64_t)p.splits * I * p.ldp * 4) : 0;
-  return p;
+  const int64_t cu = cinema_cu_count(), rt = 128 / elem_size(dt), nt = up(R, rt);
+  const TileCost *cost = dt == CINEMA_DT_F32 ? COST_32 : COST_16;
+  Plan best = {};
+  double least = 0;
+  for (int c = 0; c < (dt == CINEMA_DT_F32 ? 2 : 3); ++c) {
+    const int64_t ti = up(I, cost[c].tile), tj = up(J, cost[c].tile);
+    for (int64_t s = 1; s <= 64 && (s == 1 || nt / s >= 4); s += s < 4 ? 1 : s < 16 ? 4 : 16) {
+      double us = (double)up(ti * tj * s, cu) * (up(nt, s) * cost[c].step + cost[c].fixed);
+      if (s > 1) us += 2.5 + (double)s * I * J * 8 / 4e6;
+      if (best.tile != 0 && us >= least) continue;
+      least = us;
+      best.tile = cost[c].tile;
+      best.ti = ti;
+      best.tj = tj;
+      best.per_split = up(nt, s) * rt;
+    }
+  }
+  best.splits = (int)up(R, best.per_split);
+  best.ldp = (J + 7) & ~(int64_t)7;
+  best.part_bytes = best.splits > 1 ? align256((int64_t)best.splits * I * best.ldp * 4) : 0;
+  return best;
 }
 
-template <typename T, bool CA, bool CB, int BI, int BJ, int WI, int WJ, bool DMA>
+template <typename T, bool CA, bool CB, int BI, int BJ, int WI, int WJ>
 int launch_tile(const GemmOperand &A, const GemmOperand &B, const Epilogue &e, const Plan &p, hipStream_t st) {
-  typedef GemmTile<T, CA, CB, BI, BJ, WI, WJ, DMA> G;
-  auto fn = k_linear<T, CA, CB, BI, BJ, WI, WJ, DMA>;
+  typedef GemmTile<T, CA, CB, BI, BJ, WI, WJ> G;
+  auto fn = k_linear<T, CA, CB, BI, BJ, WI, WJ>;
   CINEMA_SMEM_ATTR(fn, G::SMEM);
   hipLaunchKernelGGL(fn, dim3((unsigned)(p.ti * p.tj), (unsigned)p.splits), dim3(WI * WJ * 64), G::SMEM, st, A, B, e, (int)p.ti, (int)p.tj, p.per_split);
   CINEMA_CHECK_HIP(hipGetLastError());
   return 0;
 }
 
-// 256 x 256 tiles (one workgroup of eight waves on a compute unit) ask the L2 for half the bytes of 128 x 128 tiles (two
-// workgroups of four waves): taken where they do not leave more of the last round empty
-bool large_tiles(int64_t I, int64_t J) {
-  const int64_t cu = cinema_cu_count();
-  return up(up(I, 256) * up(J, 256), cu) * 4 <= up(up(I, 128) * up(J, 128), 2 * cu) * 2;
+// an operand that the products read in place: rows of whole, aligned chunks, less than 2^20 values apart (32-bit offsets)
+bool whole_chunks(const void *p, int64_t ld, int64_t cols, int dt) {
+  const int64_t v = 16 / elem_size(dt);
+  return ((uintptr_t)p & 15) == 0 && ld % v == 0 && cols % v == 0 && ld < (1 << 20);
+}
+int64_t padded(int64_t cols, int dt) { return up(cols, 16 / elem_size(dt)) * (16 / elem_size(dt)); }
+int64_t pack_bytes(const void *p, int64_t ld, int64_t rows, int64_t cols, int dt) {
+  return whole_chunks(p, ld, cols, dt) ? 0 : align256(rows * padded(cols, dt) * elem_size(dt));
 }
 
+// x [xr][xc] and w [wr][wc] as the products read them: in place, or packed to `at` (one launch for both)
 template <typename T>
-bool whole_chunks(const GemmOperand &o, bool col) {
-  constexpr int V = 16 / sizeof(T);
-  return ((uintptr_t)o.p & 15) == 0 && o.ld % V == 0 && (col ? o.ext : o.red) % V == 0 && o.ld < (1 << 20);   // 256 rows below 2 GB
+int pack_operands(const void *&x, int64_t &ldx, int64_t xr, int64_t xc, const void *&w, int64_t &ldw, int64_t wr, int64_t wc, int dt, char *at,
+                  hipStream_t st) {
+  Pack p[2] = {};
+  int n = 0;
+  if (x != nullptr && !whole_chunks(x, ldx, xc, dt)) {
+    p[n++] = {x, at, xr, xc, ldx, padded(xc, dt)};
+    at += align256(xr * padded(xc, dt) * (int64_t)sizeof(T));
+    x = p[n - 1].dst;
+    ldx = p[n - 1].ldo;
+  }
+  if (w != nullptr && !whole_chunks(w, ldw, wc, dt)) {
+    p[n++] = {w, at, wr, wc, ldw, padded(wc, dt)};
+    w = p[n - 1].dst;
+    ldw = p[n - 1].ldo;
+  }
+  if (n == 0) return 0;
+  int64_t most = 0;
+  for (int i = 0; i < n; ++i) most = std::max(most, p[i].rows * p[i].ldo / (16 / (int64_t)sizeof(T)));
+  hipLaunchKernelGGL(k_linear_pack<T>, dim3((unsigned)std::min<int64_t>(up(most, 256), 8 * cinema_cu_count()), n), dim3(256), 0, st, p[0], p[1]);
+  CINEMA_CHECK_HIP(hipGetLastError());
+  return 0;
+}
+
+// 256 x 256: one workgroup of eight waves on a compute unit; the 16-bit types only (fp32 gains nothing from it)
+template <typename T, bool CA, bool CB>
+int launch_large(const GemmOperand &A, const GemmOperand &B, const Epilogue &e, const Plan &p, hipStream_t st) {
+  if constexpr (sizeof(T) == 2) return launch_tile<T, CA, CB, 256, 256, 2, 4>(A, B, e, p, st);
+  return -1;
 }
 
 // C = A B^T with the epilogue; part = workspace of plan.part_bytes
@@ -476,18 +555,10 @@ int product(const GemmOperand &A, const GemmOperand &B, Epilogue e, int dt, void
   const Plan p = plan_product(A.ext, B.ext, A.red, dt);
   e.ldp = p.ldp;
   e.part = p.splits > 1 ? (float *)part : nullptr;
-  const bool dma = whole_chunks<T>(A, CA) && whole_chunks<T>(B, CB);
   int rc;
-  if constexpr (sizeof(T) == 2) {
-    if (dma && p.tile == 128 && p.splits == 1 && large_tiles(A.ext, B.ext)) {
-      Plan q = p;
-      q.ti = up(A.ext, 256);
-      q.tj = up(B.ext, 256);
-      return launch_tile<T, CA, CB, 256, 256, 2, 4, true>(A, B, e, q, st);
-    }
-  }
-  if (p.tile == 128) rc = dma ? launch_tile<T, CA, CB, 128, 128, 2, 2, true>(A, B, e, p, st) : launch_tile<T, CA, CB, 128, 128, 2, 2, false>(A, B, e, p, st);
-  else rc = dma ? launch_tile<T, CA, CB, 64, 64, 2, 2, true>(A, B, e, p, st) : launch_tile<T, CA, CB, 64, 64, 2, 2, false>(A, B, e, p, st);
+  if (p.tile == 64) rc = launch_tile<T, CA, CB, 64, 64, 2, 2>(A, B, e, p, st);
+  else if (p.tile == 128 || sizeof(T) == 4) rc = launch_tile<T, CA, CB, 128, 128, 2, 2>(A, B, e, p, st);
+  else rc = launch_large<T, CA, CB>(A, B, e, p, st);
   if (rc != 0 || p.splits == 1) return rc;
   const int64_t groups = A.ext * (p.ldp >> 3);
   hipLaunchKernelGGL(k_linear_join<T>, dim3((unsigned)std::min<int64_t>(up(groups, 256), 4096)), dim3(256), 0, st, e, A.ext, B.ext, p.splits);
@@ -497,10 +568,10 @@ int product(const GemmOperand &A, const GemmOperand &B, Epilogue e, int dt, void
 
 int check_sizes(const char *who, int64_t M, int64_t K, int64_t N, int dt) {
   CINEMA_REQUIRE(dt == CINEMA_DT_F32 || dt == CINEMA_DT_BF16 || dt == CINEMA_DT_F16, "%s: unknown type %d", who, dt);
-  CINEMA_REQUIRE(M >= 1 && K >= 1 && N >= 1 && K <= (1 << 24) && N <= (1 << 24) && M <= 0x7fffffffll,
-                 "%s: need 1 <= M < 2^31 and 1 <= K, N <= 2^24 (got M = %lld, K = %lld, N = %lld)", who, (long long)M, (long long)K, (long long)N);
-  // a launch has fewer than 2^32 threads, 256 for each output tile
-  const int64_t most = (1 << 24) - 1;
+  CINEMA_REQUIRE(M >= 1 && K >= 1 && N >= 1 && K < (1 << 20) && N < (1 << 20) && M <= 0x7fffffffll,
+                 "%s: need 1 <= M < 2^31 and 1 <= K, N < 2^20 (got M = %lld, K = %lld, N = %lld)", who, (long long)M, (long long)K, (long long)N);
+  // a launch has fewer than 2^32 threads, at most 512 for each output tile
+  const int64_t most = (1 << 23) - 1;
   const Plan y = plan_product(M, N, K, dt), dx = plan_product(M, K, N, dt), dw = plan_product(N, K, M, dt);
   CINEMA_REQUIRE(y.ti * y.tj <= most && dx.ti * dx.tj <= most && dw.ti * dw.tj <= most, "%s: M = %lld, K = %lld, N = %lld need too many tiles", who,
                  (long long)M, (long long)K, (long long)N);
@@ -513,22 +584,24 @@ int64_t dz_rows(int64_t M, int64_t N) {
   return up(M, by);
 }
 
-struct BackwardPlan { int64_t dz, db, part, total; };
-BackwardPlan plan_backward(int64_t M, int64_t K, int64_t N, int dt) {
+struct BackwardPlan { int64_t ldz, dz, db, pack, part, total; };
+BackwardPlan plan_backward(const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N, int dt) {
   BackwardPlan b;
+  b.ldz = padded(N, dt);
   b.dz = 0;
-  int64_t at = align256(M * N * elem_size(dt));
-  b.db = at;
-  at += align256(up(M, dz_rows(M, N)) * N * 4);
-  b.part = at;
-  at += std::max(plan_product(M, K, N, dt).part_bytes, plan_product(N, K, M, dt).part_bytes);
-  b.total = at;
+  b.db = align256(M * b.ldz * elem_size(dt));
+  b.pack = b.db + align256(up(M, dz_rows(M, N)) * N * 4);
+  b.part = b.pack + pack_bytes(x, ldx, M, K, dt) + pack_bytes(w, K, N, K, dt);
+  b.total = b.part + std::max(plan_product(M, K, N, dt).part_bytes, plan_product(N, K, M, dt).part_bytes);
   return b;
+}
+int64_t forward_pack_bytes(const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N, int dt) {
+  return pack_bytes(x, ldx, M, K, dt) + pack_bytes(w, K, N, K, dt);
 }
 
 template <typename T>
 int forward_t(const void *x, int64_t ldx, const void *w, const void *bias, int bias_f32, const void *res, int64_t ldres, int64_t M, int64_t K,
-              int64_t N, int act, int dt, void *z, void *y, void *work, hipStream_t st) {
+              int64_t N, int act, int dt, void *z, void *y, char *work, hipStream_t st) {
   Epilogue e = {};
   e.bias = bias; e.bias_f32 = bias_f32; e.res = res; e.ldres = ldres; e.act = act; e.z = z; e.out = y;
   if (M <= ROWS_MAX) {
@@ -539,39 +612,52 @@ int forward_t(const void *x, int64_t ldx, const void *w, const void *bias, int b
     CINEMA_CHECK_HIP(hipGetLastError());
     return 0;
   }
-  const GemmOperand A = {x, ldx, M, K}, B = {w, K, N, K};
-  return product<T, false, false>(A, B, e, dt, work, st);
+  char *part = work + forward_pack_bytes(x, ldx, w, M, K, N, dt);
+  int64_t ldw = K;
+  const int rc = pack_operands<T>(x, ldx, M, K, w, ldw, N, K, dt, work, st);
+  if (rc != 0) return rc;
+  const GemmOperand A = {x, ldx, M, K}, B = {w, ldw, N, K};
+  return product<T, false, false>(A, B, e, dt, part, st);
 }
 
 template <typename T>
 int backward_t(const void *dy, const void *z, const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N, int act, int dt,
                int db_f32, void *dx, void *dw, void *db, char *work, hipStream_t st) {
-  const BackwardPlan bp = plan_backward(M, K, N, dt);
+  const BackwardPlan bp = plan_backward(x, ldx, w, M, K, N, dt);
   const void *dz = dy;
-  if (act != ACT_NONE || db != nullptr) {
+  int64_t ldz = N;
+  const bool rewrite = (dx != nullptr || dw != nullptr) && (act != ACT_NONE || !whole_chunks(dy, N, N, dt));
+  if (rewrite || db != nullptr) {
     const int64_t rows = dz_rows(M, N), P = up(M, rows);
-    T *out = act != ACT_NONE ? (T *)(work + bp.dz) : nullptr;
+    T *out = rewrite ? (T *)(work + bp.dz) : nullptr;
     float *part = db != nullptr ? (float *)(work + bp.db) : nullptr;
-    hipLaunchKernelGGL(k_linear_dz<T>, dim3((unsigned)up(N, 512), (unsigned)P), dim3(256), 0, st, (const T *)dy, z, out, part, M, N, rows, act, db,
-                       db_f32);
+    // db alone of an activation: its sums need the slope, so dz is written all the same
+    if (db != nullptr && act != ACT_NONE) out = (T *)(work + bp.dz);
+    hipLaunchKernelGGL(k_linear_dz<T>, dim3((unsigned)up(N, 512), (unsigned)P), dim3(256), 0, st, (const T *)dy, z, out, bp.ldz, part, M, N, rows, act,
+                       db, db_f32);
     CINEMA_CHECK_HIP(hipGetLastError());
-    if (out != nullptr) dz = out;
+    if (out != nullptr) { dz = out; ldz = bp.ldz; }
     if (db != nullptr && P > 1) {
       hipLaunchKernelGGL(k_column_join<T>, dim3((unsigned)up(N, 32)), dim3(1024), 0, st, part, (int)P, N, db, db_f32);
       CINEMA_CHECK_HIP(hipGetLastError());
     }
   }
+  int64_t ldw = K;
+  if (dx == nullptr) w = nullptr;
+  if (dw == nullptr) x = nullptr;
+  int rc = pack_operands<T>(x, ldx, M, K, w, ldw, N, K, dt, work + bp.pack, st);
+  if (rc != 0) return rc;
   Epilogue e = {};
   if (dx != nullptr) {
     e.out = dx;
-    const GemmOperand A = {dz, N, M, N}, B = {w, K, K, N};
-    const int rc = product<T, false, true>(A, B, e, dt, work + bp.part, st);
+    const GemmOperand A = {dz, ldz, M, N}, B = {w, ldw, K, N};
+    rc = product<T, false, true>(A, B, e, dt, work + bp.part, st);
     if (rc != 0) return rc;
   }
   if (dw != nullptr) {
     e.out = dw;
-    const GemmOperand A = {dz, N, N, M}, B = {x, ldx, K, M};
-    const int rc = product<T, true, true>(A, B, e, dt, work + bp.part, st);
+    const GemmOperand A = {dz, ldz, N, M}, B = {x, ldx, K, M};
+    rc = product<T, true, true>(A, B, e, dt, work + bp.part, st);
     if (rc != 0) return rc;
   }
   return 0;
@@ -579,10 +665,11 @@ int backward_t(const void *dy, const void *z, const void *x, int64_t ldx, const 
 
 }  // namespace
 
-extern "C" int64_t cinema_linear_work_bytes(int64_t M, int64_t K, int64_t N, int32_t dtype, int32_t backward) {
+extern "C" int64_t cinema_linear_work_bytes(const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N, int32_t dtype,
+                                            int32_t backward) {
   if (check_sizes("cinema_linear_work_bytes", M, K, N, dtype) != 0) return -1;
-  if (backward) return plan_backward(M, K, N, dtype).total;
-  return M <= ROWS_MAX ? 0 : plan_product(M, N, K, dtype).part_bytes;
+  if (backward) return plan_backward(x, ldx, w, M, K, N, dtype).total;
+  return M <= ROWS_MAX ? 0 : forward_pack_bytes(x, ldx, w, M, K, N, dtype) + plan_product(M, N, K, dtype).part_bytes;
 }
 
 extern "C" int cinema_linear_forward(const void *x, int64_t ldx, const void *w, const void *bias, int32_t bias_f32, const void *res, int64_t ldres,
@@ -590,11 +677,11 @@ extern "C" int cinema_linear_forward(const void *x, int64_t ldx, const void *w, 
   if (check_sizes("cinema_linear_forward", M, K, N, dtype) != 0) return -1;
   CINEMA_REQUIRE(x && w && y && ldx >= K && (!res || ldres >= N), "cinema_linear_forward: null operand, or a row stride below the row");
   CINEMA_REQUIRE(act >= 0 && act < ACT_COUNT, "cinema_linear_forward: unknown activation %d", act);
-  CINEMA_REQUIRE(work || cinema_linear_work_bytes(M, K, N, dtype, 0) == 0, "cinema_linear_forward: null workspace");
+  CINEMA_REQUIRE(work || cinema_linear_work_bytes(x, ldx, w, M, K, N, dtype, 0) == 0, "cinema_linear_forward: null workspace");
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == CINEMA_DT_F32) return forward_t<float>(x, ldx, w, bias, 1, res, ldres, M, K, N, act, dtype, z, y, work, st);
-  if (dtype == CINEMA_DT_BF16) return forward_t<bf16_t>(x, ldx, w, bias, bias_f32, res, ldres, M, K, N, act, dtype, z, y, work, st);
-  return forward_t<f16_t>(x, ldx, w, bias, bias_f32, res, ldres, M, K, N, act, dtype, z, y, work, st);
+  if (dtype == CINEMA_DT_F32) return forward_t<float>(x, ldx, w, bias, 1, res, ldres, M, K, N, act, dtype, z, y, (char *)work, st);
+  if (dtype == CINEMA_DT_BF16) return forward_t<bf16_t>(x, ldx, w, bias, bias_f32, res, ldres, M, K, N, act, dtype, z, y, (char *)work, st);
+  return forward_t<f16_t>(x, ldx, w, bias, bias_f32, res, ldres, M, K, N, act, dtype, z, y, (char *)work, st);
 }
 
 extern "C" int cinema_linear_backward(const void *dy, const void *z, const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N,

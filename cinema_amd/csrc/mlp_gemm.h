@@ -61,25 +61,10 @@ __device__ __forceinline__ void copy_to_lds(const void *base, unsigned off, unsi
                : "=&s"(keep) : "v"(off), "s"(base), "s"(lds) : "memory");
 }
 
-template <typename T>
-__device__ __forceinline__ u32x4 load_chunk(const T *p, int n) {   // n valid values, the others read as zero
-  constexpr int V = 16 / sizeof(T);
-  u32x4 r = {0u, 0u, 0u, 0u};
-  if (n >= V) {
-    __builtin_memcpy(&r, p, 16);        // 2- or 4-byte aligned: one dwordx4 in the target's unaligned mode
-  } else if (n > 0) {
-    T e[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) e[k] = k < n ? p[k] : (T)0.f;
-    __builtin_memcpy(&r, e, 16);
-  }
-  return r;
-}
-
-// One operand of a workgroup's tile: NROW rows of i, copied by NW waves.  DMA: chunks are whole and 16-byte aligned
-// (ld, ext of COL, red of ROW are multiples of a chunk) and go to LDS directly; otherwise they pass through registers, value
-// by value where a chunk is cut by an end.
-template <typename T, bool COL, int NROW, int NW, bool DMA>
+// One operand of a workgroup's tile: NROW rows of i, copied by NW waves.  Its chunks are whole and 16-byte aligned: p and ld are
+// multiples of a chunk, and so is the row's length, or the row is followed by zeros up to the next multiple (linear.hip packs
+// operands that are neither).
+template <typename T, bool COL, int NROW, int NW>
 struct TileCopy {
   static constexpr int V = 16 / sizeof(T);
   static constexpr int RT = 128 / sizeof(T);                          // values of r in a tile
@@ -88,14 +73,10 @@ struct TileCopy {
   static constexpr int NC = BYTES / 1024 / NW;                        // 1024-byte pieces per wave
   static_assert(NC >= 1 && BYTES % (1024 * NW) == 0, "tile too small for this many waves");
   const T *base;            // first value of the workgroup's rows (ROW) or columns (COL) in the next tile; wave-uniform
-  int64_t off[DMA ? 1 : NC];
-  unsigned off32[DMA ? NC : 1];   // bytes from base; the host takes DMA only where a tile spans less than 2 GB
+  unsigned off[NC];         // bytes from base: below 2 GB, as rows are less than 2^20 values apart
   int chunk0[NC];           // r of the chunk's first value inside a tile
-  int nvalid[DMA ? 1 : NC]; // COL: values of i in the chunk that exist
-  u32x4 st[DMA ? 1 : NC];
-  int64_t step;             // elements from tile to tile
+  int64_t step;             // values from tile to tile
   int64_t left;             // values of r from the next tile on
-  bool whole;               // COL: no chunk of the workgroup is cut by the end of i
 
   __device__ static __forceinline__ int key(int row) {
     // 64 banks: 16 lanes of a 16-byte read, 32 lanes of an 8-byte read and 64 lanes of a 4-byte read share a cycle
@@ -106,57 +87,28 @@ struct TileCopy {
   __device__ __forceinline__ void init(const GemmOperand &o, int64_t i0, int64_t r0, int64_t r1, int wave, int lane) {
     left = r1 - r0;
     step = COL ? (int64_t)RT * o.ld : RT;
-    whole = !COL || i0 + NROW <= o.ext;
     base = (const T *)o.p + (COL ? r0 * o.ld + i0 : i0 * o.ld + r0);
 #pragma unroll
     for (int q = 0; q < NC; ++q) {
       const int c = ((wave * NC + q) * 64 + lane);                    // chunk number in the image
       const int row = c / CPR, ch = (c % CPR) ^ key(row);
-      int64_t at;
-      if (COL) {
-        const int64_t n = o.ext - (i0 + ch * V);
-        at = (int64_t)row * o.ld + (n > 0 ? ch * V : 0);
-        chunk0[q] = row;
-        if (!DMA) nvalid[q] = n <= 0 ? 0 : (n < V ? (int)n : V);
-      } else {
-        const int64_t last = o.ext - 1 - i0;                          // rows past the end repeat the last: never stored
-        at = (row < last ? row : last) * o.ld + ch * V;
-        chunk0[q] = ch * V;
-        if (!DMA) nvalid[q] = V;
-      }
-      if (DMA) off32[q] = (unsigned)at * (unsigned)sizeof(T);
-      else off[q] = at;
+      // rows and columns past the end repeat one that exists: their products are never stored
+      const int64_t last = o.ext - 1 - i0;
+      const int64_t at = COL ? (int64_t)row * o.ld + (ch * V <= last ? ch * V : 0) : (row < last ? row : last) * o.ld + ch * V;
+      chunk0[q] = COL ? row : ch * V;
+      off[q] = (unsigned)at * (unsigned)sizeof(T);
     }
   }
-  // DMA: piece q of the next tile.  WHOLE: the tile is whole in r; else what is past the end comes as zeros.
+  // piece q of the next tile.  WHOLE: the tile is whole in r; else chunks past the end come as zeros
   template <bool WHOLE>
   __device__ __forceinline__ void copy(int q, unsigned lds, int wave) const {
     const unsigned to = lds + (unsigned)(wave * NC + q) * 1024u;
-    if (WHOLE) copy_to_lds(base, off32[q], to);
-    else copy_to_lds(left > chunk0[q] ? (const void *)((const char *)base + off32[q]) : (const void *)&g_zero_chunk, to);
+    if (WHOLE) copy_to_lds(base, off[q], to);
+    else copy_to_lds(left > chunk0[q] ? (const void *)((const char *)base + off[q]) : (const void *)&g_zero_chunk, to);
   }
   __device__ __forceinline__ void advance() {
     base += step;
     left -= RT;
-  }
-  // through registers
-  __device__ __forceinline__ void load() {
-    if (left >= RT && whole) {                                        // uniform
-#pragma unroll
-      for (int q = 0; q < NC; ++q) __builtin_memcpy(&st[DMA ? 0 : q], base + off[DMA ? 0 : q], 16);
-    } else {
-#pragma unroll
-      for (int q = 0; q < NC; ++q) {
-        const int64_t n = left - chunk0[q];
-        st[DMA ? 0 : q] = load_chunk(base + off[DMA ? 0 : q], n <= 0 ? 0 : (COL ? nvalid[DMA ? 0 : q] : (n < V ? (int)n : V)));
-      }
-    }
-    base += step;
-    left -= RT;
-  }
-  __device__ __forceinline__ void store(lds_char *tile, int wave, int lane) {
-#pragma unroll
-    for (int q = 0; q < NC; ++q) *(LDS_AS u32x4 *)(tile + ((wave * NC + q) * 64 + lane) * 16) = st[DMA ? 0 : q];
   }
   // fragment of rows i..i+31 of the tile, chunk pair kk
   __device__ static __forceinline__ typename Mma<T>::frag frag(const lds_char *tile, int i, int kk, int lane) {
@@ -201,11 +153,11 @@ __device__ __forceinline__ void bare_barrier() {
 // Tile of BI x BJ results on WI x WJ waves; acc[a][b] are the wave's 32 x 32 blocks.  Two LDS buffers, one barrier per tile of
 // r: it publishes the copies of tile t and frees the other buffer for those of tile t + 1, which run while tile t is
 // multiplied.  Fragments are read one step (two chunks of r) ahead of the matrix instructions.
-template <typename T, bool CA, bool CB, int BI, int BJ, int WI, int WJ, bool DMA>
+template <typename T, bool CA, bool CB, int BI, int BJ, int WI, int WJ>
 struct GemmTile {
   static constexpr int NW = WI * WJ, TI = BI / WI / 32, TJ = BJ / WJ / 32;
-  typedef TileCopy<T, CA, BI, NW, DMA> LA;
-  typedef TileCopy<T, CB, BJ, NW, DMA> LB;
+  typedef TileCopy<T, CA, BI, NW> LA;
+  typedef TileCopy<T, CB, BJ, NW> LB;
   typedef typename Mma<T>::frag F;
   static constexpr int STAGE = LA::BYTES + LB::BYTES;
   static constexpr int SMEM = 2 * STAGE;
@@ -279,42 +231,17 @@ struct GemmTile {
     lb.init(B, j0, r0, r1, wave, lane);
     const int nt = (int)((r1 - r0 + RT - 1) / RT);
     if (nt <= 0) return;
-    if constexpr (DMA) {
 #pragma unroll
-      for (int q = 0; q < LA::NC; ++q) la.template copy<false>(q, lds0, wave);
+    for (int q = 0; q < LA::NC; ++q) la.template copy<false>(q, lds0, wave);
 #pragma unroll
-      for (int q = 0; q < LB::NC; ++q) lb.template copy<false>(q, lds0 + LA::BYTES, wave);
-      la.advance();
-      lb.advance();
-      int t = 0;
-      const int whole = (int)((r1 - r0) / RT) - 1;          // tiles whose successor is whole
-      for (; t < whole; ++t) tile<1>(acc, la, lb, t, base, lds0, wi, wj, lane, wave);
-      for (; t < nt - 1; ++t) tile<2>(acc, la, lb, t, base, lds0, wi, wj, lane, wave);
-      tile<0>(acc, la, lb, t, base, lds0, wi, wj, lane, wave);
-    } else {
-      la.load();
-      lb.load();
-      la.store(base, wave, lane);
-      lb.store(base + LA::BYTES, wave, lane);
-      for (int t = 0; t < nt; ++t) {
-        lds_char *cur = base + (t & 1) * STAGE, *nxt = base + ((t & 1) ^ 1) * STAGE;
-        __syncthreads();        // tile t is there for every wave, and every wave is done with tile t - 1
-        if (t + 1 < nt) {
-          la.load();
-          lb.load();
-        }
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          Frags f;
-          read(f, cur, kk, wi, wj, lane);
-          multiply(acc, f);
-        }
-        if (t + 1 < nt) {
-          la.store(nxt, wave, lane);
-          lb.store(nxt + LA::BYTES, wave, lane);
-        }
-      }
-    }
+    for (int q = 0; q < LB::NC; ++q) lb.template copy<false>(q, lds0 + LA::BYTES, wave);
+    la.advance();
+    lb.advance();
+    int t = 0;
+    const int whole = (int)((r1 - r0) / RT) - 1;          // tiles whose successor is whole
+    for (; t < whole; ++t) tile<1>(acc, la, lb, t, base, lds0, wi, wj, lane, wave);
+    for (; t < nt - 1; ++t) tile<2>(acc, la, lb, t, base, lds0, wi, wj, lane, wave);
+    tile<0>(acc, la, lb, t, base, lds0, wi, wj, lane, wave);
     __syncthreads();            // the caller's epilogue reuses the buffers
   }
 };

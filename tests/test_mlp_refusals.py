@@ -73,11 +73,14 @@ def test_c_entry_points_check_their_arguments():
     from cinema_amd import _lib
     lib = _lib.load()
     dt = _lib.DT_BF16
-    assert lib.cinema_linear_work_bytes(25000, 512, 512, dt, 0) == 0
-    assert lib.cinema_linear_work_bytes(25000, 512, 512, dt, 1) >= 25000 * 512 * 2
-    for bad in [(0, 8, 8, dt), (8, 0, 8, dt), (8, 8, -1, dt), (8, 8, 8, 3), (1 << 31, 8, 8, dt), (8, 1 << 25, 8, dt), (1 << 30, 8, 1 << 20, dt)]:
+    x = C.c_void_p(1 << 20)
+    assert lib.cinema_linear_work_bytes(x, 512, x, 25000, 512, 512, dt, 0) == 0
+    assert lib.cinema_linear_work_bytes(x, 512, x, 25000, 512, 512, dt, 1) >= 25000 * 512 * 2
+    assert lib.cinema_linear_work_bytes(x, 511, x, 25000, 511, 512, dt, 0) >= 25000 * 512 * 2        # packed rows
+    assert lib.cinema_linear_work_bytes(C.c_void_p((1 << 20) + 2), 512, x, 25000, 512, 512, dt, 0) >= 25000 * 512 * 2
+    for bad in [(0, 8, 8, dt), (8, 0, 8, dt), (8, 8, -1, dt), (8, 8, 8, 3), (1 << 31, 8, 8, dt), (8, 1 << 20, 8, dt), (1 << 30, 8, 1 << 19, dt)]:
         for back in (0, 1):
-            assert lib.cinema_linear_work_bytes(*bad, back) == -1
+            assert lib.cinema_linear_work_bytes(x, 8, x, *bad, back) == -1
         assert b"cinema_linear" in lib.cinema_last_error()
     one = C.c_void_p(256)
     ok = [one, 8, one, None, 0, None, 0, 16, 8, 8, 0, dt, None, one, None, None]
