@@ -23,57 +23,69 @@ __device__ __forceinline__ float row_sum(float x, float *red, int slot) {
   return t;
 }
 
-// NW == 1: four rows per workgroup of four waves; else one row per workgroup of NW waves
+// NW == 1: a workgroup of four waves, each with its own rows; else a workgroup of NW waves on one row after the other.  Weights
+// stay in registers over the rows (read per row they would be as many bytes from the L2 as the rows from memory), and the
+// next row is under way while this one is reduced.  
 template <typename T, typename W, int NW, int CH>
 __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void k_norm_fwd(const T *x, int64_t ldx, const W *w, const W *b, int64_t M, int D, float eps,
                                                                       T *y, float *mean, float *rstd) {
   constexpr int V = Piece<T>::V, LANES = NW * 64;
-  __shared__ float red[3 * (NW == 1 ? 1 : NW)];
+  __shared__ float red[4 * (NW == 1 ? 1 : NW)];
   const int lane = NW == 1 ? (threadIdx.x & 63) : threadIdx.x;
-  const int64_t row = NW == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  const int64_t step = (int64_t)gridDim.x * (NW == 1 ? 4 : 1);
+  int64_t row = NW == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
   if (row >= M) return;
-  float v[CH][V];
-  float s = 0.f;
+  float wv[CH][V], bv[CH][V];
+  u32x4 next[CH];
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int k = (c * LANES + lane) * V;
-    load_piece(x + row * ldx + k, D - k, v[c]);
+    next[c] = load_raw(x + row * ldx + k, D - k);
 #pragma unroll
-    for (int q = 0; q < V; ++q) s += v[c][q];
+    for (int q = 0; q < V; ++q) { wv[c][q] = 1.f; bv[c][q] = 0.f; }
+    if (w != nullptr) load_values<W, V>(w + k, D - k, wv[c]);
+    if (b != nullptr) load_values<W, V>(b + k, D - k, bv[c]);
   }
-  const float mu = row_sum<NW>(s, red, 0) / (float)D;
-  float q2 = 0.f;
+  int slot = 0;
+  for (; row < M; row += step) {
+    float v[CH][V];
+    float s = 0.f;
 #pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    const int k = (c * LANES + lane) * V;
+    for (int c = 0; c < CH; ++c) {
+      raw_values<T>(next[c], v[c]);
 #pragma unroll
-    for (int q = 0; q < V; ++q) {
-      v[c][q] = k + q < D ? v[c][q] - mu : 0.f;
-      q2 += v[c][q] * v[c][q];
+      for (int q = 0; q < V; ++q) s += v[c][q];
     }
-  }
-  const float rs = 1.f / sqrtf(row_sum<NW>(q2, red, 1) / (float)D + eps);
-  if (mean != nullptr && lane == 0) { mean[row] = mu; rstd[row] = rs; }
+    if (row + step < M) {
 #pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    const int k = (c * LANES + lane) * V, n = D - k;
-    if (n <= 0) continue;
-    float o[V];
-#pragma unroll
-    for (int q = 0; q < V; ++q) o[q] = v[c][q] * rs;
-    if (w != nullptr) {
-      float a[V];
-      load_values<W, V>(w + k, n, a);
-#pragma unroll
-      for (int q = 0; q < V; ++q) o[q] *= a[q];
+      for (int c = 0; c < CH; ++c) {
+        const int k = (c * LANES + lane) * V;
+        next[c] = load_raw(x + (row + step) * ldx + k, D - k);
+      }
     }
-    if (b != nullptr) {
-      float a[V];
-      load_values<W, V>(b + k, n, a);
+    const float mu = row_sum<NW>(s, red, slot) / (float)D;        // divided: a constant row has its mean exactly
+    float q2 = 0.f;
 #pragma unroll
-      for (int q = 0; q < V; ++q) o[q] += a[q];
+    for (int c = 0; c < CH; ++c) {
+      const int k = (c * LANES + lane) * V;
+#pragma unroll
+      for (int q = 0; q < V; ++q) {
+        v[c][q] = k + q < D ? v[c][q] - mu : 0.f;
+        q2 = fmaf(v[c][q], v[c][q], q2);
+      }
     }
-    store_piece(y + row * (int64_t)D + k, n, o);
+    const float rs = 1.f / sqrtf(row_sum<NW>(q2, red, slot + 1) / (float)D + eps);
+    slot ^= 2;                                  // a row's sums are read before the row after the next writes there
+    if (mean != nullptr && lane == 0) { mean[row] = mu; rstd[row] = rs; }
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int k = (c * LANES + lane) * V, n = D - k;
+      if (n <= 0) continue;
+      float o[V];
+#pragma unroll
+      for (int q = 0; q < V; ++q) o[q] = fmaf(v[c][q] * rs, wv[c][q], bv[c][q]);
+      store_piece(y + row * (int64_t)D + k, n, o);
+    }
   }
 }
 
@@ -142,26 +154,41 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void k_norm_bwd(const T *g
     if (w != nullptr) load_values<W, V>(w + k, D - k, wv[c]);
   }
   int slot = 0;
-  for (int64_t row = (int64_t)blockIdx.x * RPW + (NW == 1 ? wave : 0); row < M; row += (int64_t)gridDim.x * RPW) {
-    const float mu = mean[row], rs = rstd[row];
+  const int64_t step = (int64_t)gridDim.x * RPW;
+  int64_t row = (int64_t)blockIdx.x * RPW + (NW == 1 ? wave : 0);
+  u32x4 nx[CH], ng[CH];                         // the next row, under way while this one is reduced
+  float nmu = 0.f, nrs = 0.f;
+  auto fetch = [&](int64_t r) {
+    nmu = mean[r];
+    nrs = rstd[r];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int k = (c * LANES + lane) * V;
+      nx[c] = load_raw(x + r * ldx + k, D - k);
+      ng[c] = load_raw(g + r * (int64_t)D + k, D - k);
+    }
+  };
+  if (row < M) fetch(row);
+  for (; row < M; row += step) {
+    const float mu = nmu, rs = nrs;
     float h[CH][V], gv[CH][V];
     float c1 = 0.f, c2 = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int k = (c * LANES + lane) * V;
-      load_piece(x + row * ldx + k, D - k, h[c]);
-      load_piece(g + row * (int64_t)D + k, D - k, gv[c]);
+      raw_values<T>(nx[c], h[c]);
+      raw_values<T>(ng[c], gv[c]);
     }
+    if (row + step < M) fetch(row + step);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int k = (c * LANES + lane) * V;
 #pragma unroll
       for (int q = 0; q < V; ++q) {
         h[c][q] = k + q < D ? (h[c][q] - mu) * rs : 0.f;
-        if (PARAMS) { sw[c][q] += gv[c][q] * h[c][q]; sb[c][q] += gv[c][q]; }
+        if (PARAMS) { sw[c][q] = fmaf(gv[c][q], h[c][q], sw[c][q]); sb[c][q] += gv[c][q]; }
         gv[c][q] *= wv[c][q];
         c1 += gv[c][q];
-        c2 += gv[c][q] * h[c][q];
+        c2 = fmaf(gv[c][q], h[c][q], c2);
       }
     }
     if (dx == nullptr) continue;
@@ -181,7 +208,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void k_norm_bwd(const T *g
       if (n <= 0) continue;
       float o[V];
 #pragma unroll
-      for (int q = 0; q < V; ++q) o[q] = rs * (gv[c][q] - c1 - h[c][q] * c2);
+      for (int q = 0; q < V; ++q) o[q] = rs * fmaf(-h[c][q], c2, gv[c][q] - c1);
       store_piece(dx + row * (int64_t)D + k, n, o);
     }
   }
@@ -279,21 +306,23 @@ __global__ __launch_bounds__(256) void k_norm_params_long(const T *g, const T *x
   part[(int64_t)blockIdx.y * 2 * D + D + k] = b;
 }
 
-// dw | db = sum of P rows of partials [P][2][D] in a fixed order; 64 columns per workgroup, sixteen waves over the partials
+// dw | db = sum of P rows of partials [P][2][D] in a fixed order: 32 columns per workgroup, 32 groups of lanes over the partials
 template <typename W>
 __global__ __launch_bounds__(1024) void k_norm_join(const float *part, int P, int64_t D, W *dw, W *db) {
-  __shared__ float red[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t col = (int64_t)blockIdx.x * 64 + lane;
+  __shared__ float red[32][33];
+  const int c = threadIdx.x & 31, grp = threadIdx.x >> 5;
+  const int64_t col = (int64_t)blockIdx.x * 32 + c;
   float s = 0.f;
-  if (col < 2 * D)
-    for (int p = wave; p < P; p += 16) s += part[(int64_t)p * 2 * D + col];
-  red[wave][lane] = s;
+  if (col < 2 * D) {
+#pragma unroll 8
+    for (int p = grp; p < P; p += 32) s += part[(int64_t)p * 2 * D + col];
+  }
+  red[grp][c] = s;
   __syncthreads();
-  if (wave != 0 || col >= 2 * D) return;
+  if (threadIdx.x >= 32 || col >= 2 * D) return;
   float t = 0.f;
 #pragma unroll
-  for (int v = 0; v < 16; ++v) t += red[v][lane];
+  for (int g = 0; g < 32; ++g) t += red[g][c];
   if (col < D) {
     if (dw != nullptr) dw[col] = (W)t;
   } else if (db != nullptr) {
@@ -310,11 +339,17 @@ Shape shape_of(int64_t D, int es) {
   const int64_t pieces = up(D * es, 16);
   if (pieces <= 64) return {1, 1};
   if (pieces <= 128) return {1, 2};
-  if (pieces <= 256) return {1, 4};
+  if (pieces <= 256) return {4, 1};
   if (pieces <= 512) return {4, 2};
-  if (pieces <= 1024) return {4, 4};
+  if (pieces <= 1024) return {8, 2};
   if (pieces <= 2048) return {8, 4};
   return {0, 0};
+}
+
+// workgroups of the forward pass: as many as run at once, the rows dealt evenly
+int64_t fwd_blocks(int64_t M, const Shape &s) {
+  const int64_t groups = s.nw == 1 ? up(M, 4) : M, most = (int64_t)cinema_cu_count() * (s.nw == 8 ? 4 : 8);
+  return up(groups, up(groups, most));
 }
 
 // workgroups of the backward pass = rows of partials
@@ -323,7 +358,7 @@ int64_t bwd_blocks(int64_t M, int64_t D, int es) {
   const int cu = cinema_cu_count();
   if (s.nw == 0) return std::max<int64_t>(1, std::min<int64_t>(up(M, 32), 64));
   if (s.nw == 1) return std::max<int64_t>(1, std::min<int64_t>(up(M, 16), 2 * cu));
-  return std::max<int64_t>(1, std::min<int64_t>(up(M, 4), s.nw == 4 ? 2 * cu : cu));
+  return std::max<int64_t>(1, std::min<int64_t>(up(M, 4), s.nw == 4 ? 3 * cu : cu));
 }
 
 template <typename T, typename W>
@@ -331,13 +366,13 @@ int forward_t(const void *x, int64_t ldx, const void *w, const void *b, int64_t 
               hipStream_t st) {
   const Shape s = shape_of(D, sizeof(T));
 #define NORM_FWD(NW, CH)                                                                                                            \
-  hipLaunchKernelGGL((k_norm_fwd<T, W, NW, CH>), dim3((unsigned)(NW == 1 ? up(M, 4) : M)), dim3(NW == 1 ? 256 : NW * 64), 0, st,   \
+  hipLaunchKernelGGL((k_norm_fwd<T, W, NW, CH>), dim3((unsigned)fwd_blocks(M, s)), dim3(NW == 1 ? 256 : NW * 64), 0, st,             \
                      (const T *)x, ldx, (const W *)w, (const W *)b, M, (int)D, eps, (T *)y, mean, rstd)
   if (s.nw == 1 && s.ch == 1) NORM_FWD(1, 1);
-  else if (s.nw == 1 && s.ch == 2) NORM_FWD(1, 2);
-  else if (s.nw == 1) NORM_FWD(1, 4);
-  else if (s.nw == 4 && s.ch == 2) NORM_FWD(4, 2);
-  else if (s.nw == 4) NORM_FWD(4, 4);
+  else if (s.nw == 1) NORM_FWD(1, 2);
+  else if (s.nw == 4 && s.ch == 1) NORM_FWD(4, 1);
+  else if (s.nw == 4) NORM_FWD(4, 2);
+  else if (s.nw == 8 && s.ch == 2) NORM_FWD(8, 2);
   else if (s.nw == 8) NORM_FWD(8, 4);
   else hipLaunchKernelGGL((k_norm_fwd_long<T, W>), dim3((unsigned)M), dim3(1024), 0, st, (const T *)x, ldx, (const W *)w, (const W *)b, D, eps, (T *)y, mean, rstd);
 #undef NORM_FWD
@@ -372,10 +407,10 @@ int backward_t(const void *g, const void *x, int64_t ldx, const void *w, const f
   const int64_t blocks = bwd_blocks(M, D, sizeof(T));
   int rc = 0;
   if (s.nw == 1 && s.ch == 1) rc = launch_bwd<T, W, 1, 1>(g, x, ldx, w, mean, rstd, M, D, dx, dw, db, part, blocks, st);
-  else if (s.nw == 1 && s.ch == 2) rc = launch_bwd<T, W, 1, 2>(g, x, ldx, w, mean, rstd, M, D, dx, dw, db, part, blocks, st);
-  else if (s.nw == 1) rc = launch_bwd<T, W, 1, 4>(g, x, ldx, w, mean, rstd, M, D, dx, dw, db, part, blocks, st);
-  else if (s.nw == 4 && s.ch == 2) rc = launch_bwd<T, W, 4, 2>(g, x, ldx, w, mean, rstd, M, D, dx, dw, db, part, blocks, st);
-  else if (s.nw == 4) rc = launch_bwd<T, W, 4, 4>(g, x, ldx, w, mean, rstd, M, D, dx, dw, db, part, blocks, st);
+  else if (s.nw == 1) rc = launch_bwd<T, W, 1, 2>(g, x, ldx, w, mean, rstd, M, D, dx, dw, db, part, blocks, st);
+  else if (s.nw == 4 && s.ch == 1) rc = launch_bwd<T, W, 4, 1>(g, x, ldx, w, mean, rstd, M, D, dx, dw, db, part, blocks, st);
+  else if (s.nw == 4) rc = launch_bwd<T, W, 4, 2>(g, x, ldx, w, mean, rstd, M, D, dx, dw, db, part, blocks, st);
+  else if (s.nw == 8 && s.ch == 2) rc = launch_bwd<T, W, 8, 2>(g, x, ldx, w, mean, rstd, M, D, dx, dw, db, part, blocks, st);
   else if (s.nw == 8) rc = launch_bwd<T, W, 8, 4>(g, x, ldx, w, mean, rstd, M, D, dx, dw, db, part, blocks, st);
   else {
     if (dx != nullptr) hipLaunchKernelGGL((k_norm_bwd_long<T, W>), dim3((unsigned)M), dim3(1024), 0, st, (const T *)g, (const T *)x, ldx, (const W *)w, mean, rstd, D, (T *)dx);
@@ -384,7 +419,7 @@ int backward_t(const void *g, const void *x, int64_t ldx, const void *w, const f
     CINEMA_CHECK_HIP(hipGetLastError());
   }
   if (rc != 0 || !params || (s.nw != 0 && blocks == 1)) return rc;
-  hipLaunchKernelGGL(k_norm_join<W>, dim3((unsigned)up(2 * D, 64)), dim3(1024), 0, st, part, (int)blocks, D, (W *)dw, (W *)db);
+  hipLaunchKernelGGL(k_norm_join<W>, dim3((unsigned)up(2 * D, 32)), dim3(1024), 0, st, part, (int)blocks, D, (W *)dw, (W *)db);
   CINEMA_CHECK_HIP(hipGetLastError());
   return 0;
 }
