@@ -244,7 +244,7 @@ __device__ __forceinline__ void write_tile(const f32x16 (&acc)[G::TI][G::TJ], in
       for (int k = 0; k < 4; ++k) { v[k] = a[k]; v[4 + k] = b[k]; }
       if (FULL || (i < I && n > 0)) {
         if (e.part != nullptr) {
-          store8(e.part + ((int64_t)blockIdx.y * I + i) * e.ldp + j, 8, v);   // ldp is a multiple of 8
+          store8(e.part + i * e.ldp + j, 8, v);   // ldp is a multiple of 8
         } else {
           if (e.res != nullptr) {
 #pragma unroll
@@ -265,14 +265,17 @@ __global__ __launch_bounds__(WI *WJ * 64, 2) void k_linear(GemmOperand A, GemmOp
   typedef GemmTile<T, CA, CB, BI, BJ, WI, WJ> G;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // tiles that share rows of A follow each other on one XCD (its L2 then holds them): blocks of 8 row tiles, row tile fastest
-  const int id = xcd_remap(blockIdx.x, tiles_i * tiles_j);
+  // Workgroups in the order of their data: an XCD gets consecutive ids (its L2 then holds what they share), the tiles of one split
+  // after each other, in blocks of 8 row tiles with the row tile fastest.
+  const int tiles = tiles_i * tiles_j, all = xcd_remap(blockIdx.x, gridDim.x);
+  const int split = all / tiles, id = all - split * tiles;
   constexpr int GRP = 8;
   const int grp = id / (GRP * tiles_j), in = id % (GRP * tiles_j);
   const int rows = tiles_i - grp * GRP < GRP ? tiles_i - grp * GRP : GRP;
   const int64_t i0 = (int64_t)(grp * GRP + in % rows) * BI, j0 = (int64_t)(in / rows) * BJ;
-  const int64_t r0 = (int64_t)blockIdx.y * per_split;
+  const int64_t r0 = (int64_t)split * per_split;
   const int64_t r1 = r0 + per_split < A.red ? r0 + per_split : A.red;
+  if (e.part != nullptr) e.part += (int64_t)split * A.ext * e.ldp;
   f32x16 acc[G::TI][G::TJ];             // starts from the bias of the lane's column (splits: k_linear_join adds it)
 #pragma unroll
   for (int y = 0; y < G::TJ; ++y) {
@@ -387,22 +390,46 @@ __global__ __launch_bounds__(256) void k_linear_dz(const T *dy, const void *zv, 
   float sum[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) sum[k] = 0.f;
-  if (n > 0)
-    for (int64_t m = m0 + wave; m < m1; m += 4) {
-      float g[8];
-      load8(dy + m * N + j, n, g);
-      if (dz != nullptr) {
-        if (act != ACT_NONE) {
-          float z[8];
-          load8((const Z *)zv + m * N + j, n, z);
-          slope8<sizeof(T) == 2>(g, z, act);
-          if (n < 8)
-            for (int k = n; k < 8; ++k) g[k] = 0.f;                   // 0 * slope of nothing
+  auto row = [&](int64_t m, float (&g)[8], const float (&z)[8]) {
+    if (dz != nullptr) {
+      if (act != ACT_NONE) {
+        slope8<sizeof(T) == 2>(g, z, act);
+        if (n < 8) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) g[k] = k < n ? g[k] : 0.f;      // not 0 * slope of nothing
         }
-        store8(dz + m * ldz + j, ldz - j < 8 ? (int)(ldz - j) : 8, g);
+      }
+      store8(dz + m * ldz + j, ldz - j < 8 ? (int)(ldz - j) : 8, g);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum[k] += g[k];
+  };
+  const bool kept = dz != nullptr && act != ACT_NONE;
+  int64_t m = m0 + wave;
+  if (n == 8) {
+    for (; m + 12 < m1; m += 16) {                                    // four rows under way
+      T gr[4][8];
+      Z zr[4][8];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        __builtin_memcpy(gr[u], dy + (m + 4 * u) * N + j, sizeof(gr[u]));
+        if (kept) __builtin_memcpy(zr[u], (const Z *)zv + (m + 4 * u) * N + j, sizeof(zr[u]));
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) sum[k] += k < n ? g[k] : 0.f;
+      for (int u = 0; u < 4; ++u) {
+        float g[8], z[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { g[k] = (float)gr[u][k]; z[k] = kept ? (float)zr[u][k] : 0.f; }
+        row(m + 4 * u, g, z);
+      }
+    }
+  }
+  if (n > 0)
+    for (; m < m1; m += 4) {
+      float g[8], z[8];
+      load8(dy + m * N + j, n, g);
+      if (kept) load8((const Z *)zv + m * N + j, n, z);
+      row(m, g, z);
     }
   if (part == nullptr && db == nullptr) return;
 #pragma unroll
@@ -470,7 +497,7 @@ struct Plan { int tile; int splits; int64_t per_split, ti, tj, ldp, part_bytes; 
 // but near ties.  What a step costs is the L2's rate: 16, 32, 64 KB of operands at 64 to 80 GB/s and compute unit (16-bit); fp32
 // is bound by the matrix unit.  A split writes and reads its fp32 sums once more.
 struct TileCost { int tile; double step, fixed; };
-constexpr TileCost COST_16[] = {{64, 0.2, 0.8}, {128, 0.4, 2.6}, {256, 1.2, 13.}};
+constexpr TileCost COST_16[] = {{64, 0.2, 0.8}, {128, 0.45, 2.3}, {256, 1.2, 15.}};
 constexpr TileCost COST_32[] = {{64, 0.5, 1.0}, {128, 1.8, 4.5}};
 
 Plan plan_product(int64_t I, int64_t J, int64_t R, int dt) {
@@ -481,7 +508,9 @@ Plan plan_product(int64_t I, int64_t J, int64_t R, int dt) {
   for (int c = 0; c < (dt == CINEMA_DT_F32 ? 2 : 3); ++c) {
     const int64_t ti = up(I, cost[c].tile), tj = up(J, cost[c].tile);
     for (int64_t s = 1; s <= 64 && (s == 1 || nt / s >= 4); s += s < 4 ? 1 : s < 16 ? 4 : 16) {
-      double us = (double)up(ti * tj * s, cu) * (up(nt, s) * cost[c].step + cost[c].fixed);
+      // several small tiles of the last round share a compute unit with others, a 256 x 256 one has it alone
+      const double all = (double)up(ti * tj * s, cu), rounds = cost[c].tile == 256 ? all : std::max(1., 0.5 * (all + (double)(ti * tj * s) / cu));
+      double us = rounds * (up(nt, s) * cost[c].step + cost[c].fixed);
       if (s > 1) us += 2.5 + (double)s * I * J * 8 / 4e6;
       if (best.tile != 0 && us >= least) continue;
       least = us;
@@ -502,7 +531,7 @@ int launch_tile(const GemmOperand &A, const GemmOperand &B, const Epilogue &e, c
   typedef GemmTile<T, CA, CB, BI, BJ, WI, WJ> G;
   auto fn = k_linear<T, CA, CB, BI, BJ, WI, WJ>;
   CINEMA_SMEM_ATTR(fn, G::SMEM);
-  hipLaunchKernelGGL(fn, dim3((unsigned)(p.ti * p.tj), (unsigned)p.splits), dim3(WI * WJ * 64), G::SMEM, st, A, B, e, (int)p.ti, (int)p.tj, p.per_split);
+  hipLaunchKernelGGL(fn, dim3((unsigned)(p.ti * p.tj * p.splits)), dim3(WI * WJ * 64), G::SMEM, st, A, B, e, (int)p.ti, (int)p.tj, p.per_split);
   CINEMA_CHECK_HIP(hipGetLastError());
   return 0;
 }
@@ -573,7 +602,7 @@ int check_sizes(const char *who, int64_t M, int64_t K, int64_t N, int dt) {
   // a launch has fewer than 2^32 threads, at most 512 for each output tile
   const int64_t most = (1 << 23) - 1;
   const Plan y = plan_product(M, N, K, dt), dx = plan_product(M, K, N, dt), dw = plan_product(N, K, M, dt);
-  CINEMA_REQUIRE(y.ti * y.tj <= most && dx.ti * dx.tj <= most && dw.ti * dw.tj <= most, "%s: M = %lld, K = %lld, N = %lld need too many tiles", who,
+  CINEMA_REQUIRE(y.ti * y.tj * y.splits <= most && dx.ti * dx.tj * dx.splits <= most && dw.ti * dw.tj * dw.splits <= most, "%s: M = %lld, K = %lld, N = %lld need too many tiles", who,
                  (long long)M, (long long)K, (long long)N);
   return 0;
 }
