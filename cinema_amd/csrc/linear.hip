@@ -260,9 +260,9 @@ __device__ __forceinline__ void write_tile(const f32x16 (&acc)[G::TI][G::TJ], in
 }
 
 // One workgroup = one BI x BJ tile of one split.
-template <typename T, bool CA, bool CB, int BI, int BJ, int WI, int WJ>
+template <typename T, bool CA, bool CB, int BI, int BJ, int WI, int WJ, int RING>
 __global__ __launch_bounds__(WI *WJ * 64, 2) void k_linear(GemmOperand A, GemmOperand B, Epilogue e, int tiles_i, int tiles_j, int64_t per_split) {
-  typedef GemmTile<T, CA, CB, BI, BJ, WI, WJ> G;
+  typedef GemmTile<T, CA, CB, BI, BJ, WI, WJ, RING> G;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Workgroups in the order of their data: an XCD gets consecutive ids (its L2 then holds what they share), the tiles of one split
@@ -489,7 +489,7 @@ inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t align256(int64_t b) { return (b + 255) & ~(int64_t)255; }
 inline int elem_size(int dt) { return dt == CINEMA_DT_F32 ? 4 : 2; }
 
-struct Plan { int tile; int splits; int64_t per_split, ti, tj, ldp, part_bytes; };   // tile: 64, 128 or 256
+struct Plan { int tile, splits; bool deep; int64_t per_split, ti, tj, ldp, part_bytes; };   // tile: 64, 128 or 256
 
 // Tile and number of splits by an estimate of the time in microseconds.  A compute unit takes `step` for 128 bytes of r of a
 // tile and `fixed` for a tile's start and epilogue, whether its tiles run side by side or one after the other; both were fitted
@@ -521,15 +521,19 @@ Plan plan_product(int64_t I, int64_t J, int64_t R, int dt) {
     }
   }
   best.splits = (int)up(R, best.per_split);
+  // a 16-bit workgroup alone on its compute unit waits for every tile's copies: four buffers instead of two.  One split, bf16:
+  // 512 x 512 x 4096 in 64 x 64 tiles 33 -> 16 us, 2048 x 2048 x 4096 in 128 x 128 tiles 53 -> 38 us, no difference up to
+  // 16 tiles of r; with several workgroups on a compute unit they cost room: 25000 x 512 x 512 24 -> 37 us.  fp32 gains nothing.
+  best.deep = dt != CINEMA_DT_F32 && best.ti * best.tj * best.splits <= cu && best.per_split > 16 * rt;
   best.ldp = (J + 7) & ~(int64_t)7;
   best.part_bytes = best.splits > 1 ? align256((int64_t)best.splits * I * best.ldp * 4) : 0;
   return best;
 }
 
-template <typename T, bool CA, bool CB, int BI, int BJ, int WI, int WJ>
+template <typename T, bool CA, bool CB, int BI, int BJ, int WI, int WJ, int RING>
 int launch_tile(const GemmOperand &A, const GemmOperand &B, const Epilogue &e, const Plan &p, hipStream_t st) {
-  typedef GemmTile<T, CA, CB, BI, BJ, WI, WJ> G;
-  auto fn = k_linear<T, CA, CB, BI, BJ, WI, WJ>;
+  typedef GemmTile<T, CA, CB, BI, BJ, WI, WJ, RING> G;
+  auto fn = k_linear<T, CA, CB, BI, BJ, WI, WJ, RING>;
   CINEMA_SMEM_ATTR(fn, G::SMEM);
   hipLaunchKernelGGL(fn, dim3((unsigned)(p.ti * p.tj * p.splits)), dim3(WI * WJ * 64), G::SMEM, st, A, B, e, (int)p.ti, (int)p.tj, p.per_split);
   CINEMA_CHECK_HIP(hipGetLastError());
@@ -574,7 +578,7 @@ int pack_operands(const void *&x, int64_t &ldx, int64_t xr, int64_t xc, const vo
 // 256 x 256: one workgroup of eight waves on a compute unit; the 16-bit types only (fp32 gains nothing from it)
 template <typename T, bool CA, bool CB>
 int launch_large(const GemmOperand &A, const GemmOperand &B, const Epilogue &e, const Plan &p, hipStream_t st) {
-  if constexpr (sizeof(T) == 2) return launch_tile<T, CA, CB, 256, 256, 2, 4>(A, B, e, p, st);
+  if constexpr (sizeof(T) == 2) return launch_tile<T, CA, CB, 256, 256, 2, 4, 2>(A, B, e, p, st);
   return -1;
 }
 
@@ -585,8 +589,10 @@ int product(const GemmOperand &A, const GemmOperand &B, Epilogue e, int dt, void
   e.ldp = p.ldp;
   e.part = p.splits > 1 ? (float *)part : nullptr;
   int rc;
-  if (p.tile == 64) rc = launch_tile<T, CA, CB, 64, 64, 2, 2>(A, B, e, p, st);
-  else if (p.tile == 128 || sizeof(T) == 4) rc = launch_tile<T, CA, CB, 128, 128, 2, 2>(A, B, e, p, st);
+  if (p.tile == 64 && p.deep) rc = launch_tile<T, CA, CB, 64, 64, 2, 2, sizeof(T) == 2 ? 4 : 2>(A, B, e, p, st);
+  else if (p.tile == 64) rc = launch_tile<T, CA, CB, 64, 64, 2, 2, 2>(A, B, e, p, st);
+  else if (p.tile == 128 && p.deep) rc = launch_tile<T, CA, CB, 128, 128, 2, 2, sizeof(T) == 2 ? 4 : 2>(A, B, e, p, st);
+  else if (p.tile == 128 || sizeof(T) == 4) rc = launch_tile<T, CA, CB, 128, 128, 2, 2, 2>(A, B, e, p, st);
   else rc = launch_large<T, CA, CB>(A, B, e, p, st);
   if (rc != 0 || p.splits == 1) return rc;
   const int64_t groups = A.ext * (p.ldp >> 3);

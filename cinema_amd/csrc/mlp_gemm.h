@@ -140,8 +140,9 @@ struct TileCopy {
   }
 };
 
-__device__ __forceinline__ void wait_copies() {      // this wave's copies have arrived
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+template <int N>
+__device__ __forceinline__ void wait_copies() {      // all but the last N of this wave's copies have arrived
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 // barrier alone, without waiting for this wave's own loads and stores
 __device__ __forceinline__ void bare_barrier() {
@@ -150,17 +151,17 @@ __device__ __forceinline__ void bare_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// Tile of BI x BJ results on WI x WJ waves; acc[a][b] are the wave's 32 x 32 blocks.  Two LDS buffers, one barrier per tile of
-// r: it publishes the copies of tile t and frees the other buffer for those of tile t + 1, which run while tile t is
-// multiplied.  Fragments are read one step (two chunks of r) ahead of the matrix instructions.
-template <typename T, bool CA, bool CB, int BI, int BJ, int WI, int WJ>
+// Tile of BI x BJ results on WI x WJ waves; acc[a][b] are the wave's 32 x 32 blocks.  A ring of RING LDS buffers, one barrier per
+// tile of r: it publishes the copies of tile t and frees the buffer of tile t - 1 for those of tile t + RING - 1.  Two buffers
+// where other workgroups of the compute unit fill the waits, four where there are none.  Fragments are read one step (two chunks of r) ahead of the matrix instructions.
+template <typename T, bool CA, bool CB, int BI, int BJ, int WI, int WJ, int RING>
 struct GemmTile {
   static constexpr int NW = WI * WJ, TI = BI / WI / 32, TJ = BJ / WJ / 32;
   typedef TileCopy<T, CA, BI, NW> LA;
   typedef TileCopy<T, CB, BJ, NW> LB;
   typedef typename Mma<T>::frag F;
   static constexpr int STAGE = LA::BYTES + LB::BYTES;
-  static constexpr int SMEM = 2 * STAGE;
+  static constexpr int SMEM = RING * STAGE;
   static constexpr int RT = LA::RT;
 
   struct Frags { F a[TI], b[TJ]; };
@@ -194,18 +195,19 @@ struct GemmTile {
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  // tile t is multiplied, tile t + 1 copied.  NEXT: 0 there is none, 1 it is whole in r, 2 it may be cut
+  // tile t is multiplied, tile t + RING - 1 copied.  NEXT: 1 that one is whole in r, 2 it may be cut or past the end (then zeros
+  // are copied, so that the waits can count), 0 nothing is copied
   template <int NEXT>
   __device__ static __forceinline__ void tile(f32x16 (&acc)[TI][TJ], LA &la, LB &lb, int t, lds_char *base, unsigned lds0, int wi, int wj,
                                               int lane, int wave) {
     constexpr int C = NEXT ? LA::NC + LB::NC : 0, H = (C + 1) / 2;
-    const lds_char *cur = base + (t & 1) * STAGE;
-    const unsigned to = lds0 + ((t & 1) ^ 1) * STAGE;
+    const lds_char *cur = base + (t % RING) * STAGE;
+    const unsigned to = lds0 + ((t + RING - 1) % RING) * STAGE;
     auto issue = [&](int c) {
       if (c < LA::NC) la.template copy<NEXT == 1>(c, to, wave);
       else lb.template copy<NEXT == 1>(c - LA::NC, to + LA::BYTES, wave);
     };
-    wait_copies();
+    wait_copies<(RING - 2) * (LA::NC + LB::NC)>();
     bare_barrier();
     Frags f0, f1;
     read(f0, cur, 0, wi, wj, lane);
@@ -232,16 +234,24 @@ struct GemmTile {
     const int nt = (int)((r1 - r0 + RT - 1) / RT);
     if (nt <= 0) return;
 #pragma unroll
-    for (int q = 0; q < LA::NC; ++q) la.template copy<false>(q, lds0, wave);
+    for (int t = 0; t < RING - 1; ++t) {
 #pragma unroll
-    for (int q = 0; q < LB::NC; ++q) lb.template copy<false>(q, lds0 + LA::BYTES, wave);
-    la.advance();
-    lb.advance();
+      for (int q = 0; q < LA::NC; ++q) la.template copy<false>(q, lds0 + t * STAGE, wave);
+#pragma unroll
+      for (int q = 0; q < LB::NC; ++q) lb.template copy<false>(q, lds0 + t * STAGE + LA::BYTES, wave);
+      la.advance();
+      lb.advance();
+    }
     int t = 0;
-    const int whole = (int)((r1 - r0) / RT) - 1;          // tiles whose successor is whole
+    const int whole = (int)((r1 - r0) / RT) - (RING - 1);   // tiles whose successor by RING - 1 is whole
     for (; t < whole; ++t) tile<1>(acc, la, lb, t, base, lds0, wi, wj, lane, wave);
-    for (; t < nt - 1; ++t) tile<2>(acc, la, lb, t, base, lds0, wi, wj, lane, wave);
-    tile<0>(acc, la, lb, t, base, lds0, wi, wj, lane, wave);
+    if constexpr (RING == 2) {
+      for (; t < nt - 1; ++t) tile<2>(acc, la, lb, t, base, lds0, wi, wj, lane, wave);
+      tile<0>(acc, la, lb, t, base, lds0, wi, wj, lane, wave);
+    } else {
+      for (; t < nt; ++t) tile<2>(acc, la, lb, t, base, lds0, wi, wj, lane, wave);
+    }
+    wait_copies<0>();
     __syncthreads();            // the caller's epilogue reuses the buffers
   }
 };
