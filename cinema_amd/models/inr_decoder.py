@@ -52,15 +52,45 @@ class Modulator(nn.Module):
 
 
 class LatentRegressor(nn.Module):
-    """Reference: models/inr_decoder.py:126-141 (tiny 3-layer MLP on pooled latents; off the hot path)."""
+    """Reference: models/inr_decoder.py:126-141 (tiny 3-layer MLP on pooled latents; off the hot path).  Beyond the reference's
+    constructor: `hidden` widths, `layer_norm` in front of every hidden layer, `residual` around hidden layers that keep their
+    width; `precision` None runs torch's layers on any device, 'fp32' / 'bf16' the HIP operators of models/mlp.py (GPU only):
+    one launch per layer, in 32-bit arithmetic or on bf16 rows with fp32 sums.  Parameters, their names and the result's
+    shape are the same; the result is fp32."""
 
-    def __init__(self, latent_dims):
+    def __init__(self, latent_dims, hidden=(64, 32), layer_norm=False, residual=False, precision=None):
         super().__init__()
-        self.sequence = nn.Sequential(nn.Linear(latent_dims[0], 64), nn.ReLU(), nn.Linear(64, 32), nn.ReLU(),
-                                      nn.Linear(32, 1))
+        if precision not in (None, "fp32", "bf16"):
+            raise ValueError(f"LatentRegressor: precision is None, 'fp32' or 'bf16', got {precision!r}")
+        widths = [latent_dims[0], *hidden, 1]
+        layers = []
+        for a, b in zip(widths, widths[1:]):
+            layers += [nn.Linear(a, b), nn.ReLU()]
+        self.sequence = nn.Sequential(*layers[:-1])
+        self.norms = nn.ModuleList([nn.LayerNorm(a) for a in widths[:-2]]) if layer_norm else None
+        self.residual = residual
+        self.precision = precision
 
     def forward(self, latent_vecs):
-        return self.sequence(latent_vecs)
+        if self.precision is None and self.norms is None and not self.residual:
+            return self.sequence(latent_vecs)
+        linears = list(self.sequence)[::2]
+        x = latent_vecs
+        if self.precision is None:
+            for k, lin in enumerate(linears[:-1]):
+                h = torch.relu(lin(x if self.norms is None else self.norms[k](x)))
+                x = x + h if self.residual and lin.in_features == lin.out_features else h
+            return linears[-1](x)
+        from .mlp import layer_norm, linear_act
+        dtype = torch.bfloat16 if self.precision == "bf16" else torch.float32
+        x = x.to(dtype)
+        with torch.autocast("cuda", enabled=False):
+            for k, lin in enumerate(linears):
+                last = k + 1 == len(linears)
+                y = x if self.norms is None or last else layer_norm(x, self.norms[k].weight, self.norms[k].bias, self.norms[k].eps)
+                keep = x if self.residual and not last and lin.in_features == lin.out_features else None
+                x = linear_act(y, lin.weight.to(dtype), lin.bias, keep, "none" if last else "relu")
+        return x.float()
 
 
 class INR_Decoder(nn.Module):

@@ -127,6 +127,18 @@ def allreduce_sum(t: torch.Tensor, process_group=None) -> torch.Tensor:
     return t
 
 
+def union_grad_norm(table_norm: torch.Tensor, shared_norm: Optional[torch.Tensor], process_group=None) -> torch.Tensor:
+    """2-norm of the union batch's gradient from a rank's two parts: `table_norm` over the tables that live on this rank,
+    `shared_norm` over the replicated parameters after their all-reduce (None: frozen).  A rank normalises its loss by the
+    union batch / number of ranks (share_batch_normaliser_), so its table gradients are that many times the union's.  One
+    all-reduce of 4 bytes; equal on every rank."""
+    _, world = world_info(process_group)
+    square = allreduce_sum((table_norm.reshape(1) / world) ** 2, process_group)
+    if shared_norm is not None:
+        square = square + shared_norm.reshape(1) ** 2
+    return square.sqrt().reshape(())
+
+
 _HOST_STAGE: Dict[tuple, torch.Tensor] = {}
 
 

@@ -25,7 +25,7 @@ from . import _lib
 from . import engine as E
 from . import parallel as par
 from .models.inr_decoder import INR_Decoder
-from .optim import HipAdamW
+from .optim import HipAdamW, grad_norm
 
 
 class SubjectStore:
@@ -93,7 +93,10 @@ class HotPathTrainer:
     def __init__(self, args: dict, store: SubjectStore, device, process_group=None, split: str = "train",
                  decoder: Optional[INR_Decoder] = None, keep_grads: bool = False):
         """keep_grads=True leaves the step's gradients in lat_grad / tf_grad / eng.flat_grad for inspection; by default the
-        optimiser launch zeroes them as it consumes them (the next step then needs no zero_grad fill)."""
+        optimiser launch zeroes them as it consumes them (the next step then needs no zero_grad fill).
+        args['optimizer']['max_grad_norm'] (optional, no counterpart in the reference): the step's gradients -- latents,
+        transformations, conditions and the decoder together, of all ranks -- are clipped to this 2-norm in the update;
+        `opt_local.grad_norm` is the last step's norm (device tensor)."""
         import torch.distributed as dist
         self.args, self.store, self.device, self.split = args, store, torch.device(device), split
         self.pg = process_group
@@ -150,11 +153,12 @@ class HotPathTrainer:
         mlp_group = {"params": [self.flat_param] + self.conv_params, "lr": o["lr_inr"], "weight_decay": o["inr_weight_decay"]}
         if self.train_mlp and self.world == 1:
             # one process: nothing to wait for between the table-side and the MLP update -> one launch for all groups
-            self.opt_local = HipAdamW(groups + [mlp_group], clear_grads=not self.keep_grads)
+            self.opt_local = HipAdamW(groups + [mlp_group], clear_grads=not self.keep_grads, max_grad_norm=o.get("max_grad_norm"))
             self.opt_mlp = None
         else:
-            self.opt_local = HipAdamW(groups, clear_grads=not self.keep_grads)
-            self.opt_mlp = HipAdamW([mlp_group], clear_grads=not self.keep_grads) if self.train_mlp else None
+            self.opt_local = HipAdamW(groups, clear_grads=not self.keep_grads, max_grad_norm=o.get("max_grad_norm"))
+            self.opt_mlp = HipAdamW([mlp_group], clear_grads=not self.keep_grads, max_grad_norm=o.get("max_grad_norm")) \
+                if self.train_mlp else None
         self._base_lrs = [[g["lr"] for g in opt.param_groups] for opt in (self.opt_local, self.opt_mlp) if opt is not None]
         self._build_schedulers()
         self.sums = torch.zeros(4, device=self.device)
@@ -309,12 +313,7 @@ class HotPathTrainer:
             self.tfs.grad = self.tf_grad
         if self.cond_param is not None:
             self.cond_param.grad = self.cond_grad if use_ng else self._cond_table_grad(subj, dcond, n, grouped)
-        self.opt_local.step()
-        for w in [work] + work_conv:
-            if w is not None:
-                w.wait()
-        if self.opt_mlp is not None:
-            self.opt_mlp.step()
+        self._optimise([work] + work_conv)
         if self.train_mlp and not self.keep_grads:
             eng.grads_clean = True                   # the clearing AdamW consumed and zeroed flat_grad
         self.n_last, self.lo_last = n, lo
@@ -411,14 +410,27 @@ class HotPathTrainer:
             self.tfs.grad = self.tf_grad
         if self.cond_param is not None:
             self.cond_param.grad = self._cond_table_grad(subj, dcond, n, True)
-        self.opt_local.step()
-        if work is not None:
-            work.wait()
-        if self.opt_mlp is not None:
-            self.opt_mlp.step()
+        self._optimise([work])
         if self.train_mlp and not self.keep_grads:
             eng.grads_clean = True
         self.n_last, self.lo_last = n, lo
+
+    def _optimise(self, works):
+        """The update; `works`: handles of the shared gradients' all-reduces (None: already there).  A rank of several updates its
+        tables while they run -- unless the step is clipped: the norm is over everything, so it waits for them first."""
+        clipped = self.opt_local.max_grad_norm is not None and self.world > 1
+        norm = None
+        if not clipped:
+            self.opt_local.step()
+        for w in works:
+            if w is not None:
+                w.wait()
+        if clipped:
+            of = lambda opt: grad_norm([p for g in opt.param_groups for p in g["params"]])
+            norm = par.union_grad_norm(of(self.opt_local), None if self.opt_mlp is None else of(self.opt_mlp), self.pg)
+            self.opt_local.step(grad_norm=norm)
+        if self.opt_mlp is not None:
+            self.opt_mlp.step(grad_norm=norm)
 
     def _build_schedulers(self):
         """build_atlas.py:455-457: fresh CosineAnnealingLR objects on the configured learning rates (also after a checkpoint

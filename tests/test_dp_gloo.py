@@ -227,3 +227,24 @@ def _collect_worker(rank):
 
 def test_collect_jobs_brings_round_robin_volumes_to_rank_0_in_order():
     _run(_collect_worker)
+
+
+# ------------------------------------------------------------------ clipping over ranks
+def _union_norm_worker(rank):
+    g = torch.Generator().manual_seed(5)
+    tables, shared = [torch.randn(40 + 7 * r, generator=g) for r in range(WORLD)], torch.randn(90, generator=g)
+    # a rank's table gradients are WORLD times the union batch's, the all-reduced ones are the union's
+    got = par.union_grad_norm((tables[rank] * WORLD).norm(), shared.norm())
+    want = torch.cat(tables + [shared]).double().norm()
+    assert got.shape == () and abs(float(got) - float(want)) <= float(want) * 2.0 ** -20
+    frozen = par.union_grad_norm((tables[rank] * WORLD).norm(), None)
+    want = torch.cat(tables).double().norm()
+    assert abs(float(frozen) - float(want)) <= float(want) * 2.0 ** -20
+
+
+def test_union_grad_norm_over_two_ranks():
+    _run(_union_norm_worker)
+
+
+def test_union_grad_norm_of_one_process():
+    assert float(par.union_grad_norm(torch.tensor(3.0), torch.tensor(4.0))) == 5.0

@@ -612,3 +612,97 @@ def test_two_streams_at_once():
                 got.append(torch.autograd.grad(linear_act(x, w, b, r, "silu"), [x, w], dy))
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for g, v in zip(got, want) for p, q in zip(g, v))
+
+
+# ---- the framework's own callers --------------------------------------------------------------------------------------------
+def regressor_pair(precision, **kw):
+    """the regressor on the HIP operators, and the same parameters in torch's layers in 64 bits"""
+    from cinema_amd.models.inr_decoder import LatentRegressor
+    torch.manual_seed(11)
+    own = LatentRegressor([256, 3, 3, 3], precision=precision, **kw).cuda()
+    ref = LatentRegressor([256, 3, 3, 3], **kw).cuda().double()
+    ref.load_state_dict(own.state_dict())
+    return own, ref
+
+
+@pytest.mark.parametrize("kw", [{}, {"hidden": (64, 64, 32), "layer_norm": True, "residual": True}])
+@pytest.mark.parametrize("precision,tol", [("fp32", 2e-6), ("bf16", 3e-2)])
+@pytest.mark.parametrize("rows", [1, 64, 300])
+def test_latent_regressor_runs_the_operators(rows, precision, tol, kw):
+    """three or four layers deep: outputs and gradients in units of their largest value.  fp32: each layer's sums are within
+    256 * 2^-24 of their magnitudes in the worst case, a tenth of that in practice for random signs -- 2e-6 allows 2^-19.  bf16:
+    weights, rows and gradients are rounded by up to 2^-8 five times along the deepest path (5 * 2^-8 = 2e-2), plus the kinks"""
+    own, ref = regressor_pair(precision, **kw)
+    x = 0.5 + torch.randn(rows, 256, device="cuda")
+    dy = torch.randn(rows, 1, device="cuda")
+    xo, xr = x.clone().requires_grad_(True), x.double().requires_grad_(True)
+    yo, yr = own(xo), ref(xr)
+    assert yo.dtype == torch.float32 and yo.shape == (rows, 1)
+    assert float((yo.detach().double() - yr.detach()).abs().max()) <= tol * max(float(yr.detach().abs().max()), 1.0)
+    yo.backward(dy)
+    yr.backward(dy.double())
+    assert set(own.state_dict()) == set(ref.state_dict())
+    if precision == "fp32":
+        for (n, p), q in zip(own.named_parameters(), ref.parameters()):
+            assert float((p.grad.double() - q.grad).abs().max()) <= 20 * tol * max(float(q.grad.abs().max()), 1e-3), n
+    else:
+        for (n, p), q in zip(own.named_parameters(), ref.parameters()):        # relu's kinks move single entries: the 2-norm
+            assert float((p.grad.double() - q.grad).norm()) <= 0.1 * float(q.grad.norm()) + 1e-6, n
+
+
+def test_latent_regressor_trains_with_clipping():
+    """the set as it is used: norm, layers, residual, clipped AdamW -- gradients arrive, the norm is the gradients' own, and the
+    parameters move as torch's clip + AdamW move them from the same gradients"""
+    from cinema_amd.optim import HipAdamW
+    own, _ = regressor_pair("fp32", hidden=(64, 64, 32), layer_norm=True, residual=True)
+    opt = HipAdamW(own.parameters(), lr=1e-3, max_grad_norm=0.5)
+    twin = [torch.nn.Parameter(p.detach().clone()) for p in own.parameters()]
+    topt = torch.optim.AdamW(twin, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2)
+    x, t = torch.randn(64, 256, device="cuda"), 10 * torch.randn(64, 1, device="cuda")
+    for _ in range(3):
+        opt.zero_grad()
+        ((own(x) - t) ** 2).mean().backward()
+        for p, q in zip(own.parameters(), twin):
+            q.grad = p.grad.clone()
+        want = torch.nn.utils.clip_grad_norm_(twin, 0.5)
+        opt.step()
+        topt.step()
+        assert float(want) > 0.5 and abs(float(opt.grad_norm) - float(want)) <= 1e-5 * float(want)
+        for p, q in zip(own.parameters(), twin):
+            # an update is at most about lr; the two factors and moments differ by a few 2^-24 relative
+            assert float((p.detach() - q.detach()).abs().max()) <= 1e-3 * 1e-3 + float(q.detach().abs().max()) * 2.0 ** -22
+            q.data.copy_(p.detach())
+
+
+@pytest.mark.parametrize("split", ["train", "val"])
+def test_trainer_clips_the_whole_step(split):
+    """args['optimizer']['max_grad_norm']: the norm over all tables and the decoder, and the update of clipped gradients"""
+    from cinema_amd.trainer import HotPathTrainer, SubjectStore
+    from test_gpu_trainer import base_args
+    outs = []
+    for limit in (None, 1e-3):
+        args = base_args([32, 3, 3, 3], 64, 2, [1], [1, 4], 1 if split == "val" else 0, "fp32")
+        if limit is not None:
+            args["optimizer"]["max_grad_norm"] = limit
+        torch.manual_seed(0)
+        store = SubjectStore.synthetic(3, (16, 16, 16), 155.0 / 16, [155, 155, 155], 1, 4, seed=3, device="cuda:0",
+                                       cond_dims=1 if split == "val" else 0)
+        store.shuffle(torch.Generator(device="cuda").manual_seed(1))
+        tr = HotPathTrainer(args, store, "cuda:0", split=split, keep_grads=True)
+        before = [p.detach().clone() for g in tr.opt_local.param_groups for p in g["params"]]
+        tr.step(0, 500)
+        params = [p for g in tr.opt_local.param_groups for p in g["params"]]
+        outs.append((tr, before, params, [p.grad.clone() for p in params]))
+    (tr0, _, _, g0), (tr, before, params, grads) = outs
+    for a, b in zip(g0, grads):
+        # the gradients stay as they were; the trainer's fp32 kernels add with atomics, two runs agree to their parity bound
+        assert float((a - b).abs().max()) <= 1e-4 * float(a.abs().max())
+    total = float(torch.cat([g.double().flatten() for g in grads]).norm())
+    assert tr0.opt_local.grad_norm is None
+    assert total > 1e-3 and abs(float(tr.opt_local.grad_norm) - total) <= total * 2.0 ** -22
+    for p, b, g, grp in zip(params, before, grads, [gr for gr in tr.opt_local.param_groups for _ in gr["params"]]):
+        q = torch.nn.Parameter(b.clone())
+        q.grad = g * (1e-3 / (total + 1e-6))
+        torch.optim.AdamW([q], lr=grp["lr"], weight_decay=grp["weight_decay"]).step()
+        # first step: lr * g / (|g| + eps) with eps = 1e-8; where |g| is near eps the factor's 2^-22 moves it by as much
+        assert float((p.detach() - q.detach()).abs().max()) <= grp["lr"] * 2e-5 + float(b.abs().max()) * 2.0 ** -22
