@@ -357,7 +357,7 @@ int64_t bwd_blocks(int64_t M, int64_t D, int es) {
   const Shape s = shape_of(D, es);
   const int cu = cinema_cu_count();
   if (s.nw == 0) return std::max<int64_t>(1, std::min<int64_t>(up(M, 32), 64));
-  if (s.nw == 1) return std::max<int64_t>(1, std::min<int64_t>(up(M, 16), 2 * cu));
+  if (s.nw == 1) return M <= 64 ? 1 : std::min<int64_t>(up(M, 16), 2 * cu);      // one leaves dw and db finished
   return std::max<int64_t>(1, std::min<int64_t>(up(M, 4), s.nw == 4 ? 3 * cu : cu));
 }
 

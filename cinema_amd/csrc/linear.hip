@@ -318,13 +318,17 @@ __global__ __launch_bounds__(256) void k_linear_join(Epilogue e, int64_t I, int6
   }
 }
 
-// Few rows: bound by reading W once.  A wave owns FPW rows of W (output features) at a time, its lanes share the reduction
-// 16 bytes at a time; x (at most MAXM rows) comes from the cache.
+// Few rows: bound by reading W once.  A wave owns FPW rows of W (output features) and MR rows of x at a time, its lanes share the
+// reduction 16 bytes at a time; x comes from the cache.  Small products of more rows too, blockIdx.y counting groups of MR: their
+// time is that of one trip to memory, which the tiles make twice (64 x 256 x 64 fp32: 7.5 us in a tile).
 template <typename T, int MR, int FPW>
 __global__ __launch_bounds__(256) void k_linear_rows(const T *x, int64_t ldx, const T *w, int M, int64_t K, int64_t N, Epilogue e) {
   constexpr int V = 16 / sizeof(T);
   typedef typename Kept<T>::type Z;
   const int lane = threadIdx.x & 63;
+  const int64_t m0 = (int64_t)blockIdx.y * MR;
+  x += m0 * ldx;
+  M -= (int)m0;
   const int64_t f0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * FPW;
   if (f0 >= N) return;
   float s[FPW][MR];
@@ -352,27 +356,37 @@ __global__ __launch_bounds__(256) void k_linear_rows(const T *x, int64_t ldx, co
 #pragma unroll
         for (int q = 0; q < V; ++q) s[f][m] += (float)wv[f][q] * (float)xv[m][q];
   }
+  // the wave's sums, each in a lane of its own
+  constexpr int NV = MR * FPW;
+  static_assert(NV == 16 || (NV == 2 && MR == 1), "one of the two reductions below");
+  float z;
+  int at;
+  if constexpr (NV == 16) {               // lane 16 * g + i ends with value reduce16_index(i)
+    float v16[16];
 #pragma unroll
-  for (int f = 0; f < FPW; ++f)
+    for (int n = 0; n < 16; ++n) v16[n] = s[n / MR][n % MR];
+    z = reduce16_scatter(v16, lane);
+    z += __shfl_xor(z, 16, 64);
+    z += __shfl_xor(z, 32, 64);
+    at = reduce16_index(lane & 15);
+  } else {
 #pragma unroll
-    for (int m = 0; m < MR; ++m)
-#pragma unroll
-      for (int d = 32; d > 0; d >>= 1) s[f][m] += __shfl_xor(s[f][m], d, 64);
-#pragma unroll
-  for (int f = 0; f < FPW; ++f)
-#pragma unroll
-    for (int m = 0; m < MR; ++m)
-      if (lane == f * MR + m && m < M && f0 + f < N) {
-        const int64_t j = f0 + f, o = (int64_t)m * N + j;
-        float z = s[f][m];
-        if (e.bias != nullptr) z += e.bias_f32 ? ((const float *)e.bias)[j] : (float)((const T *)e.bias)[j];
-        if (e.z != nullptr) ((Z *)e.z)[o] = (Z)kept_value(z, e.act);
-        float v[8] = {z, z, z, z, z, z, z, z};
-        act8<sizeof(T) == 2>(v, e.act);
-        float y = v[0];
-        if (e.res != nullptr) y += (float)((const T *)e.res)[(int64_t)m * e.ldres + j];
-        ((T *)e.out)[o] = (T)y;
-      }
+    for (int d = 32; d > 0; d >>= 1) {
+      s[0][0] += __shfl_xor(s[0][0], d, 64);
+      s[1][0] += __shfl_xor(s[1][0], d, 64);
+    }
+    z = lane == 0 ? s[0][0] : s[1][0];
+    at = lane;
+  }
+  const int f = at / MR, m = at % MR;
+  if (lane >= NV || m >= M || f0 + f >= N) return;
+  const int64_t j = f0 + f, o = (m0 + m) * N + j;
+  if (e.bias != nullptr) z += e.bias_f32 ? ((const float *)e.bias)[j] : (float)((const T *)e.bias)[j];
+  if (e.z != nullptr) ((Z *)e.z)[o] = (Z)kept_value(z, e.act);
+  float v[8] = {z, z, z, z, z, z, z, z};
+  act8<sizeof(T) == 2>(v, e.act);
+  if (e.res != nullptr) v[0] += (float)((const T *)e.res)[(m0 + m) * e.ldres + j];
+  ((T *)e.out)[o] = (T)v[0];
 }
 
 // dz = dy * act'(z) and the column sums of dz over the block's rows.  A workgroup takes 512 columns (64 lanes x 8) and `rows`
@@ -483,8 +497,6 @@ __global__ __launch_bounds__(1024) void k_column_join(const float *part, int P, 
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
-constexpr int ROWS_MAX = 8;            // at most so many rows go to k_linear_rows
-
 inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t align256(int64_t b) { return (b + 255) & ~(int64_t)255; }
 inline int elem_size(int dt) { return dt == CINEMA_DT_F32 ? 4 : 2; }
@@ -496,6 +508,16 @@ struct Plan { int tile, splits; bool deep; int64_t per_split, ti, tj, ldp, part_
 // to 25000 x 512, 8192 x 1280, 2048 x 2048 and 32768 x 4096 outputs over r = 64 .. 4096, and tell the fastest tile there in all
 // but near ties.  What a step costs is the L2's rate: 16, 32, 64 KB of operands at 64 to 80 GB/s and compute unit (16-bit); fp32
 // is bound by the matrix unit.  A split writes and reads its fp32 sums once more.
+// Products that go to k_linear_rows: up to 8 rows, and small ones with at most so many waves that all of them run at once.
+// Rows against tiles in us: fp32 64 x 256 x 64 3.1 and 7.5, 1000 x 256 x 64 4.4 and 7.8, 512 x 512 x 512 14 and 11; bf16 (whose
+// tiles are faster, and whose short rows leave lanes idle) 64 x 1024 x 512 4.8 and 7.2, 256 x 256 x 256 4.8 and 4.2, 64 x 64 x 32
+// 4.5 and 3.2; with packing saved on top 256 x 257 x 129 5.0 and 11 (fp32), 5.8 and 7.6 (bf16).
+bool by_rows(int64_t M, int64_t K, int64_t N, int dt) {
+  if (M <= 8) return true;
+  const bool f32 = dt == CINEMA_DT_F32, ragged = K % (16 / elem_size(dt)) != 0;
+  return up(M, 8) * up(N, 2) <= (f32 || ragged ? 4096 : 2048) && K * elem_size(dt) <= 4096 && (f32 || K >= 256);
+}
+
 struct TileCost { int tile; double step, fixed; };
 constexpr TileCost COST_16[] = {{64, 0.2, 0.8}, {128, 0.45, 2.3}, {256, 1.2, 15.}};
 constexpr TileCost COST_32[] = {{64, 0.5, 1.0}, {128, 1.8, 4.5}};
@@ -585,7 +607,18 @@ int launch_large(const GemmOperand &A, const GemmOperand &B, const Epilogue &e, 
 // C = A B^T with the epilogue; part = workspace of plan.part_bytes
 template <typename T, bool CA, bool CB>
 int product(const GemmOperand &A, const GemmOperand &B, Epilogue e, int dt, void *part, hipStream_t st) {
-  const Plan p = plan_product(A.ext, B.ext, A.red, dt);
+  Plan p = plan_product(A.ext, B.ext, A.red, dt);
+  // rows that are no multiple of 16 bytes: a residual's loads and z's stores take two lines each, and 64 x 64 tiles have the
+  // waves to hide that.  8191 x 1283 outputs, bf16, gelu and residual, 128 against 64: r = 256 28 -> 22 us, 512 33 -> 30,
+  // 1024 45 -> 44; z: 27 -> 23, 32 -> 30, 43 -> 43.
+  const int64_t bytes_of_r = A.red * (int64_t)sizeof(T);
+  if (sizeof(T) == 2 && p.splits == 1 && p.tile > 64 && B.ext % 8 != 0 && up(A.ext, 64) * up(B.ext, 64) < (1 << 24) &&
+      ((e.res != nullptr && bytes_of_r <= 2048) || (e.z != nullptr && bytes_of_r <= 1024))) {
+    p.tile = 64;
+    p.deep = false;
+    p.ti = up(A.ext, 64);
+    p.tj = up(B.ext, 64);
+  }
   e.ldp = p.ldp;
   e.part = p.splits > 1 ? (float *)part : nullptr;
   int rc;
@@ -613,8 +646,9 @@ int check_sizes(const char *who, int64_t M, int64_t K, int64_t N, int dt) {
   return 0;
 }
 
-// rows of dz per workgroup of k_linear_dz: enough workgroups to fill the chip, two for a compute unit
+// rows of dz per workgroup of k_linear_dz: enough workgroups to fill the chip twice; up to 128 rows one, which leaves db finished
 int64_t dz_rows(int64_t M, int64_t N) {
+  if (M <= 128) return M;
   const int64_t bx = up(N, 512), by = std::max<int64_t>(1, std::min<int64_t>(up(M, 16), up(2 * cinema_cu_count(), bx)));
   return up(M, by);
 }
@@ -639,11 +673,10 @@ int forward_t(const void *x, int64_t ldx, const void *w, const void *bias, int b
               int64_t N, int act, int dt, void *z, void *y, char *work, hipStream_t st) {
   Epilogue e = {};
   e.bias = bias; e.bias_f32 = bias_f32; e.res = res; e.ldres = ldres; e.act = act; e.z = z; e.out = y;
-  if (M <= ROWS_MAX) {
-    const unsigned g = (unsigned)up(N, 8);
-    if (M == 1) hipLaunchKernelGGL((k_linear_rows<T, 1, 2>), dim3(g), dim3(256), 0, st, (const T *)x, ldx, (const T *)w, (int)M, K, N, e);
-    else if (M <= 4) hipLaunchKernelGGL((k_linear_rows<T, 4, 2>), dim3(g), dim3(256), 0, st, (const T *)x, ldx, (const T *)w, (int)M, K, N, e);
-    else hipLaunchKernelGGL((k_linear_rows<T, 8, 2>), dim3(g), dim3(256), 0, st, (const T *)x, ldx, (const T *)w, (int)M, K, N, e);
+  if (by_rows(M, K, N, dt)) {
+    if (M == 1) hipLaunchKernelGGL((k_linear_rows<T, 1, 2>), dim3((unsigned)up(N, 8)), dim3(256), 0, st, (const T *)x, ldx, (const T *)w, (int)M, K, N, e);
+    else if (M <= 4) hipLaunchKernelGGL((k_linear_rows<T, 4, 4>), dim3((unsigned)up(N, 16)), dim3(256), 0, st, (const T *)x, ldx, (const T *)w, (int)M, K, N, e);
+    else hipLaunchKernelGGL((k_linear_rows<T, 8, 2>), dim3((unsigned)up(N, 8), (unsigned)up(M, 8)), dim3(256), 0, st, (const T *)x, ldx, (const T *)w, (int)M, K, N, e);
     CINEMA_CHECK_HIP(hipGetLastError());
     return 0;
   }
@@ -704,7 +737,7 @@ extern "C" int64_t cinema_linear_work_bytes(const void *x, int64_t ldx, const vo
                                             int32_t backward) {
   if (check_sizes("cinema_linear_work_bytes", M, K, N, dtype) != 0) return -1;
   if (backward) return plan_backward(x, ldx, w, M, K, N, dtype).total;
-  return M <= ROWS_MAX ? 0 : forward_pack_bytes(x, ldx, w, M, K, N, dtype) + plan_product(M, N, K, dtype).part_bytes;
+  return by_rows(M, K, N, dtype) ? 0 : forward_pack_bytes(x, ldx, w, M, K, N, dtype) + plan_product(M, N, K, dtype).part_bytes;
 }
 
 extern "C" int cinema_linear_forward(const void *x, int64_t ldx, const void *w, const void *bias, int32_t bias_f32, const void *res, int64_t ldres,
