@@ -99,6 +99,12 @@ void check_companion(const char *what, const char *name, const Tensor &t, const 
   TORCH_CHECK_TYPE(t.scalar_type() == x.scalar_type() || (may_be_f32 && t.scalar_type() == at::kFloat), what, ": ", name, " has type ",
                    t.scalar_type(), ", the rows ", x.scalar_type(), may_be_f32 ? " (it may be fp32)" : "");
 }
+// lazily negated views become plain tensors; forward-mode tangents would be dropped in silence
+void check_plain(const char *what, Tensor &t) {
+  if (!t.defined()) return;
+  if (t.is_neg()) t = t.resolve_neg();
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "cinema_amd ", what, ": no forward-mode derivative");
+}
 void check_gpu(const char *what, const Tensor &x) {
   TORCH_CHECK(x.is_cuda(), "cinema_amd ", what, " runs HIP kernels: the input must live on the GPU");
 }
@@ -125,7 +131,7 @@ struct LinearActBackward : public Node {
     if (task_should_compute_output(3)) got[3] = grads[0];
     if (!need_x && !need_w && !need_b) return got;
     const c10::DeviceGuard guard(grads[0].device());
-    const Tensor g = grads[0].contiguous();
+    const Tensor g = grads[0].resolve_neg().contiguous();
     const auto o = g.options();
     if (need_x) got[0] = m ? at::empty(x_shape, o) : at::zeros(x_shape, o);
     if (need_w) got[1] = m ? at::empty({n, k}, o) : at::zeros({n, k}, o);
@@ -165,6 +171,7 @@ Tensor linear_act(Tensor x, Tensor w, const MaybeTensor &bias, const MaybeTensor
     if (r.defined()) r = r.to(t);
     if (b.defined() && b.scalar_type() != at::kFloat) b = b.to(t);
   }
+  for (Tensor *t : {&x, &w, &b, &r}) check_plain(what, *t);
   check_rows(what, x);
   check_companion(what, "weight", w, x, false);
   check_companion(what, "bias", b, x, true);
@@ -232,7 +239,7 @@ struct LayerNormBackward : public Node {
     first_order_only("layer_norm");
     const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1), need_b = task_should_compute_output(2);
     const c10::DeviceGuard guard(grads[0].device());
-    const Tensor g = grads[0].contiguous();
+    const Tensor g = grads[0].resolve_neg().contiguous();
     const auto o = g.options();
     if (need_x) got[0] = m ? at::empty(x_shape, o) : at::zeros(x_shape, o);
     if (need_w) got[1] = m ? at::empty({d}, o.dtype(w_type)) : at::zeros({d}, o.dtype(w_type));
@@ -265,6 +272,7 @@ Tensor layer_norm(Tensor x, const MaybeTensor &weight, const MaybeTensor &bias, 
     if (w.defined()) w = w.to(at::kFloat);
     if (b.defined()) b = b.to(at::kFloat);
   }
+  for (Tensor *t : {&x, &w, &b}) check_plain(what, *t);
   check_rows(what, x);
   check_companion(what, "weight", w, x, true);
   check_companion(what, "bias", b, x, true);
@@ -325,6 +333,7 @@ Tensor grad_norm(const std::vector<Tensor> &grads, double norm_type, std::option
   for (size_t i = 0; i < grads.size(); ++i) {
     const Tensor &g = grads[i];
     TORCH_CHECK_TYPE(g.layout() == at::kStrided, "gradient norm: sparse gradients are not supported");
+    TORCH_CHECK_VALUE(!g.is_neg(), "gradient norm: lazily negated gradients are not supported");
     const int dt = dtype_of(g.scalar_type());
     TORCH_CHECK_TYPE(dt >= 0, "gradient norm: gradients are fp32, bf16 or fp16, got ", g.scalar_type());
     TORCH_CHECK_VALUE(g.device() == grads[0].device(),

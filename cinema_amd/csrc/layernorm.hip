@@ -357,7 +357,7 @@ int64_t bwd_blocks(int64_t M, int64_t D, int es) {
   const Shape s = shape_of(D, es);
   const int cu = cinema_cu_count();
   if (s.nw == 0) return std::max<int64_t>(1, std::min<int64_t>(up(M, 32), 64));
-  if (s.nw == 1) return M <= 64 ? 1 : std::min<int64_t>(up(M, 16), 2 * cu);      // one leaves dw and db finished
+  if (s.nw == 1) return std::min<int64_t>(up(M, 16), 2 * cu);       // one leaves dw and db finished
   return std::max<int64_t>(1, std::min<int64_t>(up(M, 4), s.nw == 4 ? 3 * cu : cu));
 }
 
@@ -426,9 +426,9 @@ int backward_t(const void *g, const void *x, int64_t ldx, const void *w, const f
 
 int check_sizes(const char *who, int64_t M, int64_t D, int dt) {
   CINEMA_REQUIRE(dt == CINEMA_DT_F32 || dt == CINEMA_DT_BF16 || dt == CINEMA_DT_F16, "%s: unknown type %d", who, dt);
-  // a launch has fewer than 2^32 threads: one workgroup of at most 1024 for a row
-  CINEMA_REQUIRE(M >= 1 && M < (1 << 22) * (int64_t)(shape_of(D, dt == CINEMA_DT_F32 ? 4 : 2).nw == 1 ? 16 : 1) && D >= 1 && D <= (1 << 24),
-                 "%s: need 1 <= D <= 2^24 and 1 <= M < 2^22 rows (2^26 for rows of at most 4 KB), got M = %lld, D = %lld", who, (long long)M, (long long)D);
+  // rows beyond the registers take a workgroup of 1024 threads each, and a launch has fewer than 2^32 threads
+  CINEMA_REQUIRE(M >= 1 && D >= 1 && D <= (1 << 24) && M <= 0x7fffffffll && (M < (1 << 22) || shape_of(D, dt == CINEMA_DT_F32 ? 4 : 2).nw != 0),
+                 "%s: need 1 <= D <= 2^24 and 1 <= M < 2^31 rows (2^22 rows of more than 32 KB), got M = %lld, D = %lld", who, (long long)M, (long long)D);
   return 0;
 }
 

@@ -72,7 +72,7 @@ __device__ __forceinline__ void slope8(float (&g)[8], const float (&zs)[8], int 
   switch (act) {
     case ACT_RELU:                                  // the kept value is the slope
 #pragma unroll
-      for (int k = 0; k < 8; ++k) g[k] *= zs[k];
+      for (int k = 0; k < 8; ++k) g[k] = zs[k] == 0.f ? 0.f : g[k] * zs[k];    // an infinite gradient behind a closed gate is no NaN
       break;
     case ACT_GELU:
 #pragma unroll
@@ -390,13 +390,13 @@ __global__ __launch_bounds__(256) void k_linear_rows(const T *x, int64_t ldx, co
 }
 
 // dz = dy * act'(z) and the column sums of dz over the block's rows.  A workgroup takes 512 columns (64 lanes x 8) and `rows`
-// rows, its four waves every fourth row; sums of the waves meet in LDS.  dz has rows of ldz values, zeros behind the N'th (the
+// rows, its eight waves every eighth row, two of them under way; sums of the waves meet in LDS.  dz has rows of ldz values, zeros behind the N'th (the
 // products read whole chunks).  dz == null: only the sums.
 template <typename T>
-__global__ __launch_bounds__(256) void k_linear_dz(const T *dy, const void *zv, T *dz, int64_t ldz, float *part, int64_t M, int64_t N, int64_t rows,
+__global__ __launch_bounds__(512) void k_linear_dz(const T *dy, const void *zv, T *dz, int64_t ldz, float *part, int64_t M, int64_t N, int64_t rows,
                                                    int act, void *db, int db_f32) {
   typedef typename Kept<T>::type Z;
-  __shared__ float red[4][512];
+  __shared__ float red[8][512];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t j = (int64_t)blockIdx.x * 512 + lane * 8;
   const int n = j >= N ? 0 : (N - j < 8 ? (int)(N - j) : 8);
@@ -421,25 +421,25 @@ __global__ __launch_bounds__(256) void k_linear_dz(const T *dy, const void *zv, 
   const bool kept = dz != nullptr && act != ACT_NONE;
   int64_t m = m0 + wave;
   if (n == 8) {
-    for (; m + 12 < m1; m += 16) {                                    // four rows under way
-      T gr[4][8];
-      Z zr[4][8];
+    for (; m + 8 < m1; m += 16) {
+      T gr[2][8];
+      Z zr[2][8];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        __builtin_memcpy(gr[u], dy + (m + 4 * u) * N + j, sizeof(gr[u]));
-        if (kept) __builtin_memcpy(zr[u], (const Z *)zv + (m + 4 * u) * N + j, sizeof(zr[u]));
+      for (int u = 0; u < 2; ++u) {
+        __builtin_memcpy(gr[u], dy + (m + 8 * u) * N + j, sizeof(gr[u]));
+        if (kept) __builtin_memcpy(zr[u], (const Z *)zv + (m + 8 * u) * N + j, sizeof(zr[u]));
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < 2; ++u) {
         float g[8], z[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) { g[k] = (float)gr[u][k]; z[k] = kept ? (float)zr[u][k] : 0.f; }
-        row(m + 4 * u, g, z);
+        row(m + 8 * u, g, z);
       }
     }
   }
   if (n > 0)
-    for (; m < m1; m += 4) {
+    for (; m < m1; m += 8) {
       float g[8], z[8];
       load8(dy + m * N + j, n, g);
       if (kept) load8((const Z *)zv + m * N + j, n, z);
@@ -449,10 +449,10 @@ __global__ __launch_bounds__(256) void k_linear_dz(const T *dy, const void *zv, 
 #pragma unroll
   for (int k = 0; k < 8; ++k) red[wave][lane * 8 + k] = sum[k];
   __syncthreads();
-  for (int c = threadIdx.x; c < 512; c += 256) {
-    const int64_t col = (int64_t)blockIdx.x * 512 + c;
-    if (col >= N) break;
-    const float t = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+  const int c = threadIdx.x;
+  const int64_t col = (int64_t)blockIdx.x * 512 + c;
+  if (col < N) {
+    const float t = ((red[0][c] + red[1][c]) + (red[2][c] + red[3][c])) + ((red[4][c] + red[5][c]) + (red[6][c] + red[7][c]));
     if (gridDim.y > 1) part[(int64_t)blockIdx.y * N + col] = t;
     else if (db_f32) ((float *)db)[col] = t;
     else ((T *)db)[col] = (T)t;
@@ -646,9 +646,9 @@ int check_sizes(const char *who, int64_t M, int64_t K, int64_t N, int dt) {
   return 0;
 }
 
-// rows of dz per workgroup of k_linear_dz: enough workgroups to fill the chip twice; up to 128 rows one, which leaves db finished
+// rows of dz per workgroup of k_linear_dz: enough workgroups to fill the chip twice; up to 64 rows one, which leaves db finished
 int64_t dz_rows(int64_t M, int64_t N) {
-  if (M <= 128) return M;
+  if (M <= 64) return M;
   const int64_t bx = up(N, 512), by = std::max<int64_t>(1, std::min<int64_t>(up(M, 16), up(2 * cinema_cu_count(), bx)));
   return up(M, by);
 }
@@ -701,7 +701,7 @@ int backward_t(const void *dy, const void *z, const void *x, int64_t ldx, const 
     float *part = db != nullptr ? (float *)(work + bp.db) : nullptr;
     // db alone of an activation: its sums need the slope, so dz is written all the same
     if (db != nullptr && act != ACT_NONE) out = (T *)(work + bp.dz);
-    hipLaunchKernelGGL(k_linear_dz<T>, dim3((unsigned)up(N, 512), (unsigned)P), dim3(256), 0, st, (const T *)dy, z, out, bp.ldz, part, M, N, rows, act,
+    hipLaunchKernelGGL(k_linear_dz<T>, dim3((unsigned)up(N, 512), (unsigned)P), dim3(512), 0, st, (const T *)dy, z, out, bp.ldz, part, M, N, rows, act,
                        db, db_f32);
     CINEMA_CHECK_HIP(hipGetLastError());
     if (out != nullptr) { dz = out; ldz = bp.ldz; }

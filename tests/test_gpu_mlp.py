@@ -614,6 +614,20 @@ def test_two_streams_at_once():
         assert all(torch.equal(p, q) for g, v in zip(got, want) for p, q in zip(g, v))
 
 
+def test_negated_views_and_infinite_gradients():
+    """lazily negated inputs count with their sign; relu's closed gates stop an infinite gradient"""
+    from cinema_amd.models.mlp import layer_norm, linear_act
+    x, w, b, r, dy = linear_data(40, 24, 32, torch.float32)
+    assert torch.equal(linear_act(torch._neg_view(x), w, b, r, "none"), linear_act(-x, w, b, r, "none"))
+    assert torch.equal(layer_norm(torch._neg_view(x)), layer_norm(-x))
+    for rows in (4, 40):
+        xg = x[:rows].clone().requires_grad_(True)
+        y = linear_act(xg, w, None, None, "relu")
+        g = torch.full_like(y, float("inf"))
+        (dx,) = torch.autograd.grad(y, xg, torch.where(y > 0, torch.ones_like(g), g))
+        assert torch.isfinite(dx).all()
+
+
 # ---- the framework's own callers --------------------------------------------------------------------------------------------
 def regressor_pair(precision, **kw):
     """the regressor on the HIP operators, and the same parameters in torch's layers in 64 bits"""

@@ -19,6 +19,8 @@ def test_linear_act_refusals():
         linear_act(x, w, b)
     with pytest.raises(RuntimeError, match="must live on the GPU"):
         linear_act(x.bfloat16(), w.bfloat16(), b)            # a 32-bit bias beside 16-bit rows is allowed
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        linear_act(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)), w, b)
     with pytest.raises(ValueError):
         LinearAct(4, 4, activation="sine")
     assert set(LinearAct(4, 6).state_dict()) == {"weight", "bias"}
@@ -97,7 +99,7 @@ def test_c_entry_points_check_their_arguments():
         a[at] = v
         assert lib.cinema_linear_backward(*a) != 0
     assert lib.cinema_layer_norm_work_bytes(100, 512, dt) > 0
-    for bad in [(0, 8, dt), (8, 0, dt), (8, 8, 5), (1 << 27, 8, dt), (1 << 22, 1 << 20, dt), (8, (1 << 24) + 1, dt)]:
+    for bad in [(0, 8, dt), (8, 0, dt), (8, 8, 5), (1 << 31, 8, dt), (1 << 22, 1 << 20, dt), (8, (1 << 24) + 1, dt)]:
         assert lib.cinema_layer_norm_work_bytes(*bad) == -1
     assert lib.cinema_layer_norm_forward(None, 8, None, None, 0, 4, 8, 1e-5, dt, one, None, None, None) != 0
     assert lib.cinema_layer_norm_forward(one, 7, None, None, 0, 4, 8, 1e-5, dt, one, None, None, None) != 0
