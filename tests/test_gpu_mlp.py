@@ -720,3 +720,68 @@ def test_trainer_clips_the_whole_step(split):
         torch.optim.AdamW([q], lr=grp["lr"], weight_decay=grp["weight_decay"]).step()
         # first step: lr * g / (|g| + eps) with eps = 1e-8; where |g| is near eps the factor's 2^-22 moves it by as much
         assert float((p.detach() - q.detach()).abs().max()) <= grp["lr"] * 2e-5 + float(b.abs().max()) * 2.0 ** -22
+
+
+# ---- far offsets --------------------------------------------------------------------------------------------------------------
+def test_linear_beyond_32_bit_offsets():
+    """y and dy of 70 000 x 32 768 values (2.3 G): the last rows and columns against the formula"""
+    from cinema_amd.models.mlp import linear_act
+    m, k, n = 70000, 8, 32768
+    x, w, b, _, _ = linear_data(m, k, n, torch.bfloat16, res=False)
+    xg, wg = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    y = linear_act(xg, wg, b, None, "silu")
+    dy = torch.empty_like(y).normal_(0, 0.1)
+    dx, dw = torch.autograd.grad(y, [xg, wg], dy)
+    want = linear_bounds(x[-64:], w, b, None, dy[-64:], "silu")
+    within(y.detach()[-64:], *want["y"], "y")
+    within(dx[-64:], *want["dx"], "dx")
+    cols = slice(n - 16, n)
+    want = linear_bounds(x, w[cols], b[cols], None, dy[:, cols], "silu")
+    within(dw[cols], *want["dw"], "dw")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_linear_longest_reduction(dtype):
+    check_linear(16, (1 << 20) - 1, 4, dtype, "silu")
+    check_linear(3, (1 << 20) - 1, 2, dtype, "none")
+
+
+def test_layer_norm_and_clip_beyond_32_bit_offsets():
+    from cinema_amd.models.mlp import layer_norm
+    from cinema_amd.optim import clip_grad_norm_
+    m, d = 530000, 4096
+    x = torch.empty(m, d, device="cuda", dtype=torch.bfloat16).normal_(0.3, 1.5).requires_grad_(True)
+    w, b = torch.ones(d, device="cuda"), torch.zeros(d, device="cuda")
+    y = layer_norm(x, w, b)
+    dy = torch.empty_like(y).normal_(0, 0.1)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    want = norm_bounds(x.detach()[-50:], w, b, dy[-50:], 1e-5)
+    within(y.detach()[-50:], *want["y"], "y")
+    within(dx[-50:], *want["dx"], "dx")
+    del x, y, dy
+    g = dx.view(-1)
+    p = torch.nn.Parameter(torch.empty(1, device="cuda", dtype=torch.bfloat16).expand(g.numel()))
+    p.grad = g
+    tail = g[-1000:].double()
+    norm = math.sqrt(sum(float(c.double().square().sum()) for c in g.split(1 << 28)))
+    assert abs(float(clip_grad_norm_(p, norm / 2)) - norm) <= norm * 2.0 ** -22
+    within(g[-1000:], tail * ((norm / 2) / (norm + 1e-6)), tail.abs() * 2.0 ** -7.9, "clipped tail")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n", [(2040, 4104, 2040), (2040, 2040, 4104), (1000, 1288, 1001), (1000, 1000, 1288), (12500, 264, 520), (25000, 512, 512)])
+def test_linear_where_a_workgroup_is_alone(m, k, n, dtype):
+    """as many tiles as compute units, long reductions: four buffers, 64 x 64 and 128 x 128, each memory order, ragged ends"""
+    check_linear(m, k, n, dtype, "gelu_tanh")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_linear_largest_tiles(dtype):
+    """256 x 256 tiles in all three products, whole and cut by the ends, with and without splits"""
+    check_linear(33000, 1032, 4104, dtype, "silu")
+    check_linear(33001, 1031, 4103, dtype, "relu", bias=False)
+
+
+def test_linear_largest_tiles_fp32():
+    check_linear(16380, 2050, 1030, torch.float32, "silu")
+    check_linear(16384, 2048, 1024, torch.float32, "gelu")
