@@ -33,17 +33,17 @@ __device__ __forceinline__ float normal_tail_hw(float z, float &e) {
 }
 constexpr float TANH_A = 0.79788456080286536f;      // sqrt(2 / pi)
 
-// act(z) of eight values; NaN stays
-template <bool HW>
-__device__ __forceinline__ void act8(float (&v)[8], int act) {
+// act(z) of C values; NaN stays
+template <bool HW, int C>
+__device__ __forceinline__ void act_values(float (&v)[C], int act) {
   switch (act) {
     case ACT_RELU:
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = v[k] < 0.f ? 0.f : v[k];
+      for (int k = 0; k < C; ++k) v[k] = v[k] < 0.f ? 0.f : v[k];
       break;
     case ACT_GELU:
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < C; ++k) {
         float e;
         const float z = v[k];
         // z q for z < 0, z - z q for z > 0, q the small side's probability; infinities: q is 0 there
@@ -53,14 +53,14 @@ __device__ __forceinline__ void act8(float (&v)[8], int act) {
       break;
     case ACT_GELU_TANH:                             // 0.5 z (1 + tanh u) = z / (1 + e^-2u)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < C; ++k) {
         const float z = v[k], u2 = z * fmaf(2.f * TANH_A * 0.044715f, z * z, 2.f * TANH_A);
         v[k] = HW ? z * sigmoid_hw(u2) : z / (1.f + expf(-u2));
       }
       break;
     case ACT_SILU:
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = HW ? v[k] * sigmoid_hw(v[k]) : v[k] / (1.f + expf(-v[k]));
+      for (int k = 0; k < C; ++k) v[k] = HW ? v[k] * sigmoid_hw(v[k]) : v[k] / (1.f + expf(-v[k]));
       break;
     default: break;
   }
@@ -187,7 +187,7 @@ __device__ __forceinline__ void finish8(const Epilogue &e, int64_t i, int64_t j,
     for (int k = 0; k < 8; ++k) h[k] = kept_value(v[k], e.act);
     store8((Z *)e.z + i * J + j, n, h);
   }
-  act8<sizeof(T) == 2>(v, e.act);
+  act_values<sizeof(T) == 2>(v, e.act);
   if (e.res != nullptr) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] += r[k];
@@ -233,26 +233,34 @@ __device__ __forceinline__ void write_tile(const f32x16 (&acc)[G::TI][G::TJ], in
         }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+    // the slab's values of a lane all at once: one branch on what the epilogue does, and the reads and stores overlap
+    float v[PASSES * 8];
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
-      const int row = p * RPP + lane / PER;
-      const int64_t i = ix + p * RPP;
-      float v[8], r[8];
-      const int s0 = ((c8 >> 2) ^ slot_key(row)) << 2;
+      const int row = p * RPP + lane / PER, s0 = ((c8 >> 2) ^ slot_key(row)) << 2;
       const f32x4 a = *(LDS_AS f32x4 *)(slab + row * WTJ + s0), b = *(LDS_AS f32x4 *)(slab + row * WTJ + (s0 ^ 4));
 #pragma unroll
-      for (int k = 0; k < 4; ++k) { v[k] = a[k]; v[4 + k] = b[k]; }
-      if (FULL || (i < I && n > 0)) {
-        if (e.part != nullptr) {
-          store8(e.part + i * e.ldp + j, 8, v);   // ldp is a multiple of 8
-        } else {
-          if (e.res != nullptr) {
+      for (int k = 0; k < 4; ++k) { v[8 * p + k] = a[k]; v[8 * p + 4 + k] = b[k]; }
+    }
+    auto store_all = [&](auto *out, int64_t ld, int width, auto value) {       // rows of `ld` values, `width` of them from column j on
 #pragma unroll
-            for (int k = 0; k < 8; ++k) r[k] = (float)res[p][k];
-          }
-          finish8<T>(e, i, j, n, J, v, r);
-        }
+      for (int p = 0; p < PASSES; ++p) {
+        float o[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] = value(8 * p + k);
+        if (FULL || ix + p * RPP < I) store8(out + (ix + p * RPP) * ld + j, FULL ? 8 : width, o);
       }
+    };
+    if (e.part != nullptr) {
+      store_all(e.part, e.ldp, n > 0 ? 8 : 0, [&](int k) { return v[k]; });    // ldp is a multiple of 8
+    } else {
+      if (e.z != nullptr) store_all((typename Kept<T>::type *)e.z, J, n, [&](int k) { return kept_value(v[k], e.act); });
+      act_values<sizeof(T) == 2>(v, e.act);
+      if (e.res != nullptr) {
+#pragma unroll
+        for (int k = 0; k < PASSES * 8; ++k) v[k] += (float)res[k / 8][k % 8];
+      }
+      store_all((T *)e.out, J, n, [&](int k) { return v[k]; });
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -383,8 +391,8 @@ __global__ __launch_bounds__(256) void k_linear_rows(const T *x, int64_t ldx, co
   const int64_t j = f0 + f, o = (m0 + m) * N + j;
   if (e.bias != nullptr) z += e.bias_f32 ? ((const float *)e.bias)[j] : (float)((const T *)e.bias)[j];
   if (e.z != nullptr) ((Z *)e.z)[o] = (Z)kept_value(z, e.act);
-  float v[8] = {z, z, z, z, z, z, z, z};
-  act8<sizeof(T) == 2>(v, e.act);
+  float v[1] = {z};
+  act_values<sizeof(T) == 2>(v, e.act);
   if (e.res != nullptr) v[0] += (float)((const T *)e.res)[(m0 + m) * e.ldres + j];
   ((T *)e.out)[o] = (T)v[0];
 }
