@@ -511,11 +511,6 @@ inline int elem_size(int dt) { return dt == CINEMA_DT_F32 ? 4 : 2; }
 
 struct Plan { int tile, splits; bool deep; int64_t per_split, ti, tj, ldp, part_bytes; };   // tile: 64, 128 or 256
 
-// Tile and number of splits by an estimate of the time in microseconds.  A compute unit takes `step` for 128 bytes of r of a
-// tile and `fixed` for a tile's start and epilogue, whether its tiles run side by side or one after the other; both were fitted
-// to 25000 x 512, 8192 x 1280, 2048 x 2048 and 32768 x 4096 outputs over r = 64 .. 4096, and tell the fastest tile there in all
-// but near ties.  What a step costs is the L2's rate: 16, 32, 64 KB of operands at 64 to 80 GB/s and compute unit (16-bit); fp32
-// is bound by the matrix unit.  A split writes and reads its fp32 sums once more.
 // Products that go to k_linear_rows: up to 8 rows, and small ones with at most so many waves that all of them run at once.
 // Rows against tiles in us: fp32 64 x 256 x 64 3.1 and 7.5, 1000 x 256 x 64 4.4 and 7.8, 512 x 512 x 512 14 and 11; bf16 (whose
 // tiles are faster, and whose short rows leave lanes idle) 64 x 1024 x 512 4.8 and 7.2, 256 x 256 x 256 4.8 and 4.2, 64 x 64 x 32
@@ -526,21 +521,27 @@ bool by_rows(int64_t M, int64_t K, int64_t N, int dt) {
   return up(M, 8) * up(N, 2) <= (f32 || ragged ? 4096 : 2048) && K * elem_size(dt) <= 4096 && (f32 || K >= 256);
 }
 
-struct TileCost { int tile; double step, fixed; };
-constexpr TileCost COST_16[] = {{64, 0.2, 0.8}, {128, 0.45, 2.3}, {256, 1.2, 15.}};
-constexpr TileCost COST_32[] = {{64, 0.5, 1.0}, {128, 1.8, 4.5}};
+// Tile and number of splits by an estimate of the time in microseconds.  A compute unit takes `step` for 128 bytes of r of a
+// tile and `fixed` for its start and epilogue -- of sums alone, with an activation, with a residual or a kept z -- whether its
+// tiles run side by side or one after the other.  All were fitted to 25000 x 512, 8192 x 1280, 2048 x 2048 and 32768 x 4096
+// outputs over r = 64 .. 4096, and tell the fastest tile there in all but near ties.  A step costs what the L2 takes for its 16,
+// 32 or 64 KB of operands (16-bit); fp32 is bound by the matrix unit.  A split writes and reads its fp32 sums once more.
+enum { EPI_SUMS = 0, EPI_ACT, EPI_HEAVY };
+struct TileCost { int tile; double step, fixed[3]; };
+constexpr TileCost COST_16[] = {{64, 0.2, {0.6, 0.9, 1.1}}, {128, 0.45, {2.1, 3.2, 4.7}}, {256, 1.4, {7., 12., 19.}}};
+constexpr TileCost COST_32[] = {{64, 0.5, {1.0, 1.3, 1.5}}, {128, 1.8, {4.5, 6.0, 7.0}}};
 
-Plan plan_product(int64_t I, int64_t J, int64_t R, int dt) {
+Plan plan_product(int64_t I, int64_t J, int64_t R, int dt, int epi) {
   const int64_t cu = cinema_cu_count(), rt = 128 / elem_size(dt), nt = up(R, rt);
   const TileCost *cost = dt == CINEMA_DT_F32 ? COST_32 : COST_16;
   Plan best = {};
   double least = 0;
   for (int c = 0; c < (dt == CINEMA_DT_F32 ? 2 : 3); ++c) {
     const int64_t ti = up(I, cost[c].tile), tj = up(J, cost[c].tile);
-    for (int64_t s = 1; s <= 64 && (s == 1 || nt / s >= 4); s += s < 4 ? 1 : s < 16 ? 4 : 16) {
-      // several small tiles of the last round share a compute unit with others, a 256 x 256 one has it alone
-      const double all = (double)up(ti * tj * s, cu), rounds = cost[c].tile == 256 ? all : std::max(1., 0.5 * (all + (double)(ti * tj * s) / cu));
-      double us = rounds * (up(nt, s) * cost[c].step + cost[c].fixed);
+    for (int64_t s = 1; s == 1 || (s <= 64 && nt >= 4 * s && ti * tj < 2 * cu); s += s < 4 ? 1 : s < 16 ? 4 : 16) {
+      // the small tiles of the last round share compute units with others'
+      const double all = (double)up(ti * tj * s, cu), rounds = cost[c].tile > 64 ? all : std::max(1., 0.5 * (all + (double)(ti * tj * s) / cu));
+      double us = rounds * (up(nt, s) * cost[c].step + cost[c].fixed[s > 1 ? EPI_SUMS : epi]);
       if (s > 1) us += 2.5 + (double)s * I * J * 8 / 4e6;
       if (best.tile != 0 && us >= least) continue;
       least = us;
@@ -554,7 +555,7 @@ Plan plan_product(int64_t I, int64_t J, int64_t R, int dt) {
   // a 16-bit workgroup alone on its compute unit waits for every tile's copies: four buffers instead of two.  One split, bf16:
   // 512 x 512 x 4096 in 64 x 64 tiles 33 -> 16 us, 2048 x 2048 x 4096 in 128 x 128 tiles 53 -> 38 us, no difference up to
   // 16 tiles of r; with several workgroups on a compute unit they cost room: 25000 x 512 x 512 24 -> 37 us.  fp32 gains nothing.
-  best.deep = dt != CINEMA_DT_F32 && best.ti * best.tj * best.splits <= cu && best.per_split > 16 * rt;
+  best.deep = dt != CINEMA_DT_F32 && best.tile < 256 && best.ti * best.tj * best.splits <= cu && best.per_split > 16 * rt;
   best.ldp = (J + 7) & ~(int64_t)7;
   best.part_bytes = best.splits > 1 ? align256((int64_t)best.splits * I * best.ldp * 4) : 0;
   return best;
@@ -615,7 +616,7 @@ int launch_large(const GemmOperand &A, const GemmOperand &B, const Epilogue &e, 
 // C = A B^T with the epilogue; part = workspace of plan.part_bytes
 template <typename T, bool CA, bool CB>
 int product(const GemmOperand &A, const GemmOperand &B, Epilogue e, int dt, void *part, hipStream_t st) {
-  Plan p = plan_product(A.ext, B.ext, A.red, dt);
+  Plan p = plan_product(A.ext, B.ext, A.red, dt, e.res != nullptr || e.z != nullptr ? EPI_HEAVY : e.act != ACT_NONE ? EPI_ACT : EPI_SUMS);
   // rows that are no multiple of 16 bytes: a residual's loads and z's stores take two lines each, and 64 x 64 tiles have the
   // waves to hide that.  8191 x 1283 outputs, bf16, gelu and residual, 128 against 64: r = 256 28 -> 22 us, 512 33 -> 30,
   // 1024 45 -> 44; z: 27 -> 23, 32 -> 30, 43 -> 43.
@@ -648,8 +649,11 @@ int check_sizes(const char *who, int64_t M, int64_t K, int64_t N, int dt) {
                  "%s: need 1 <= M < 2^31 and 1 <= K, N < 2^20 (got M = %lld, K = %lld, N = %lld)", who, (long long)M, (long long)K, (long long)N);
   // a launch has fewer than 2^32 threads, at most 512 for each output tile
   const int64_t most = (1 << 23) - 1;
-  const Plan y = plan_product(M, N, K, dt), dx = plan_product(M, K, N, dt), dw = plan_product(N, K, M, dt);
-  CINEMA_REQUIRE(y.ti * y.tj * y.splits <= most && dx.ti * dx.tj * dx.splits <= most && dw.ti * dw.tj * dw.splits <= most, "%s: M = %lld, K = %lld, N = %lld need too many tiles", who,
+  if ((up(M, 64) + 1) * (up(std::max(K, N), 64) + 1) * 64 <= most && up(K, 64) * up(N, 64) * 64 <= most) return 0;     // any plan
+  const Plan p[5] = {plan_product(M, N, K, dt, EPI_SUMS), plan_product(M, N, K, dt, EPI_ACT), plan_product(M, N, K, dt, EPI_HEAVY),
+                     plan_product(M, K, N, dt, EPI_SUMS), plan_product(N, K, M, dt, EPI_SUMS)};
+  for (const Plan &q : p)
+    CINEMA_REQUIRE(q.ti * q.tj * q.splits <= most, "%s: M = %lld, K = %lld, N = %lld need too many tiles", who,
                  (long long)M, (long long)K, (long long)N);
   return 0;
 }
@@ -669,8 +673,12 @@ BackwardPlan plan_backward(const void *x, int64_t ldx, const void *w, int64_t M,
   b.db = align256(M * b.ldz * elem_size(dt));
   b.pack = b.db + align256(up(M, dz_rows(M, N)) * N * 4);
   b.part = b.pack + pack_bytes(x, ldx, M, K, dt) + pack_bytes(w, K, N, K, dt);
-  b.total = b.part + std::max(plan_product(M, K, N, dt).part_bytes, plan_product(N, K, M, dt).part_bytes);
+  b.total = b.part + std::max(plan_product(M, K, N, dt, EPI_SUMS).part_bytes, plan_product(N, K, M, dt, EPI_SUMS).part_bytes);
   return b;
+}
+int64_t forward_part_bytes(int64_t M, int64_t K, int64_t N, int dt) {       // whatever the epilogue will be
+  return std::max({plan_product(M, N, K, dt, EPI_SUMS).part_bytes, plan_product(M, N, K, dt, EPI_ACT).part_bytes,
+                   plan_product(M, N, K, dt, EPI_HEAVY).part_bytes});
 }
 int64_t forward_pack_bytes(const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N, int dt) {
   return pack_bytes(x, ldx, M, K, dt) + pack_bytes(w, K, N, K, dt);
@@ -745,7 +753,7 @@ extern "C" int64_t cinema_linear_work_bytes(const void *x, int64_t ldx, const vo
                                             int32_t backward) {
   if (check_sizes("cinema_linear_work_bytes", M, K, N, dtype) != 0) return -1;
   if (backward) return plan_backward(x, ldx, w, M, K, N, dtype).total;
-  return by_rows(M, K, N, dtype) ? 0 : forward_pack_bytes(x, ldx, w, M, K, N, dtype) + plan_product(M, N, K, dtype).part_bytes;
+  return by_rows(M, K, N, dtype) ? 0 : forward_pack_bytes(x, ldx, w, M, K, N, dtype) + forward_part_bytes(M, K, N, dtype);
 }
 
 extern "C" int cinema_linear_forward(const void *x, int64_t ldx, const void *w, const void *bias, int32_t bias_f32, const void *res, int64_t ldres,
