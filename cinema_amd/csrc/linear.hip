@@ -468,6 +468,93 @@ __global__ __launch_bounds__(512) void k_linear_dz(const T *dy, const void *zv, 
   }
 }
 
+// Small backward passes in one launch, dz in 32 bits (few values of dz share their rounding among many gradients: it would not
+// average out).  dx and dW have one form, eight rows and 64 columns of the result per workgroup:
+//   out[i][k] = sum over r of coef[r][i] * src[r][k]      dx: r = n, coef = dz[m0 + i][n], src = W;   dW: r = m, coef = dz[m][n0 + i], src = x
+// coef comes from dy and z into LDS (a broadcast per product); blockIdx.y counts the eights of dx, then those of dW.
+constexpr int SMALL_R = 512;
+template <typename T>
+__global__ __launch_bounds__(256) void k_linear_small(const T *dy, const void *zv, const T *x, int64_t ldx, const T *w, int M, int K, int N, int act,
+                                                      T *dx, T *dw, void *db, int db_f32) {
+  typedef typename Kept<T>::type Z;
+  __shared__ __attribute__((aligned(16))) float coef[SMALL_R][8];
+  __shared__ float red[32][8], sums[4][8][64];
+  const int mb = dx != nullptr ? (M + 7) / 8 : 0;
+  const bool is_dx = (int)blockIdx.y < mb;
+  const int base = (is_dx ? blockIdx.y : blockIdx.y - mb) * 8, R = is_dx ? N : M, rows = is_dx ? M : N;
+  for (int t = threadIdx.x; t < R * 8; t += 256) {
+    // neighbouring threads read neighbouring n
+    const int i = is_dx ? t / R : t & 7, r = is_dx ? t % R : t >> 3;
+    const int m = is_dx ? base + i : r, n = is_dx ? r : base + i;
+    float g[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (m < M && n < N) {
+      g[0] = (float)dy[(int64_t)m * N + n];
+      if (act != ACT_NONE) {
+        const float z[8] = {(float)((const Z *)zv)[(int64_t)m * N + n], 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        slope8<sizeof(T) == 2>(g, z, act);
+      }
+    }
+    coef[r][i] = g[0];
+  }
+  __syncthreads();
+  // 64 columns; the four waves share r
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, k = blockIdx.x * 64 + lane;
+  const T *src = (is_dx ? w : x) + (k < K ? k : 0);
+  T *out = is_dx ? dx : dw;
+  const int64_t ld = is_dx ? K : ldx;
+  if (out != nullptr) {
+    float s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = 0.f;
+    const int per = (R + 3) >> 2, r1 = (wave + 1) * per < R ? (wave + 1) * per : R;
+    int r = wave * per;
+    for (; r + 16 <= r1; r += 16) {                 // sixteen loads under way
+      T v[16];
+#pragma unroll
+      for (int u = 0; u < 16; ++u) v[u] = src[(r + u) * ld];
+#pragma unroll
+      for (int u = 0; u < 16; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] = fmaf(coef[r + u][i], (float)v[u], s[i]);
+    }
+    for (; r + 4 <= r1; r += 4) {
+      T v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = src[(r + u) * ld];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] = fmaf(coef[r + u][i], (float)v[u], s[i]);
+    }
+    for (; r < r1; ++r) {
+      const float v = (float)src[r * ld];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] = fmaf(coef[r][i], v, s[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sums[wave][i][lane] = s[i];
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {                   // a wave stores two of the eight rows
+      const int i = 2 * wave + u;
+      const float t = (sums[0][i][lane] + sums[1][i][lane]) + (sums[2][i][lane] + sums[3][i][lane]);
+      if (base + i < rows && k < K) out[(int64_t)(base + i) * K + k] = (T)t;
+    }
+  }
+  if (is_dx || db == nullptr || blockIdx.x != 0) return;
+  const int i = threadIdx.x & 7, part = threadIdx.x >> 3;
+  float s = 0.f;
+  for (int r = part; r < R; r += 32) s += coef[r][i];
+  red[part][i] = s;
+  __syncthreads();
+  if (part != 0 || base + i >= N) return;
+  s = 0.f;
+#pragma unroll
+  for (int q = 0; q < 32; ++q) s += red[q][i];
+  if (db_f32) ((float *)db)[base + i] = s;
+  else ((T *)db)[base + i] = (T)s;
+}
+
 // 8191 x 257 fp16 with a weight of 1283 x 257: 5.4 us, mostly the trip to memory.
 // rows [R][ld] of C values -> [R][ldo], ldo the next multiple of a chunk, zeros behind; a thread moves a chunk.  Two at once.
 struct Pack { const void *src; void *dst; int64_t rows, cols, ld, ldo; };
@@ -668,6 +755,14 @@ int64_t dz_rows(int64_t M, int64_t N) {
   return up(M, by);
 }
 
+// Backward passes that go to k_linear_small.  Forward and backward kernels in us, against dz, packing, products and joins:
+// fp32 64 x 256 x 64 8 and 32, 256 x 257 x 129 17 and 34, 500 x 64 x 500 29 and 38, 512 x 512 x 512 41 and 41; bf16 64 x 256 x 64
+// 9 and 26, 64 x 1024 x 256 16 and 22, 256 x 512 x 128 17 and 17, 512 x 512 x 64 26 and 20.
+bool small_backward(int64_t M, int64_t K, int64_t N, int dt) {
+  const bool f32 = dt == CINEMA_DT_F32;
+  return std::max(M, N) <= (f32 ? SMALL_R : SMALL_R / 2) && M * K * N <= (f32 ? 32 << 20 : 17 << 20);
+}
+
 struct BackwardPlan { int64_t ldz, dz, db, pack, part, total; };
 BackwardPlan plan_backward(const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N, int dt) {
   BackwardPlan b;
@@ -710,6 +805,14 @@ int forward_t(const void *x, int64_t ldx, const void *w, const void *bias, int b
 template <typename T>
 int backward_t(const void *dy, const void *z, const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N, int act, int dt,
                int db_f32, void *dx, void *dw, void *db, char *work, hipStream_t st) {
+  if (small_backward(M, K, N, dt)) {
+    const unsigned blocks = (unsigned)((dx != nullptr ? up(M, 8) : 0) + (dw != nullptr || db != nullptr ? up(N, 8) : 0));
+    if (blocks == 0) return 0;
+    hipLaunchKernelGGL(k_linear_small<T>, dim3((unsigned)up(K, 64), blocks), dim3(256), 0, st, (const T *)dy, z, (const T *)x, ldx, (const T *)w,
+                       (int)M, (int)K, (int)N, act, (T *)dx, (T *)dw, db, db_f32);
+    CINEMA_CHECK_HIP(hipGetLastError());
+    return 0;
+  }
   const BackwardPlan bp = plan_backward(x, ldx, w, M, K, N, dt);
   const void *dz = dy;
   int64_t ldz = N;
@@ -755,7 +858,7 @@ int backward_t(const void *dy, const void *z, const void *x, int64_t ldx, const 
 extern "C" int64_t cinema_linear_work_bytes(const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N, int32_t dtype,
                                             int32_t backward) {
   if (check_sizes("cinema_linear_work_bytes", M, K, N, dtype) != 0) return -1;
-  if (backward) return plan_backward(x, ldx, w, M, K, N, dtype).total;
+  if (backward) return small_backward(M, K, N, dtype) ? 0 : plan_backward(x, ldx, w, M, K, N, dtype).total;
   return by_rows(M, K, N, dtype) ? 0 : forward_pack_bytes(x, ldx, w, M, K, N, dtype) + forward_part_bytes(M, K, N, dtype);
 }
 
@@ -775,7 +878,8 @@ extern "C" int cinema_linear_backward(const void *dy, const void *z, const void 
                                       int32_t act, int32_t dtype, int32_t db_f32, void *dx, void *dw, void *db, void *work, void *stream) {
   if (check_sizes("cinema_linear_backward", M, K, N, dtype) != 0) return -1;
   CINEMA_REQUIRE(act >= 0 && act < ACT_COUNT, "cinema_linear_backward: unknown activation %d", act);
-  CINEMA_REQUIRE(dy && (act == ACT_NONE || z) && (!dx || w) && (!dw || x) && (!dw || ldx >= K) && work, "cinema_linear_backward: null operand");
+  CINEMA_REQUIRE(dy && (act == ACT_NONE || z) && (!dx || w) && (!dw || x) && (!dw || ldx >= K), "cinema_linear_backward: null operand, or a row stride below the row");
+  CINEMA_REQUIRE(work || cinema_linear_work_bytes(x, ldx, w, M, K, N, dtype, 1) == 0, "cinema_linear_backward: null workspace");
   hipStream_t st = (hipStream_t)stream;
   if (dtype == CINEMA_DT_F32) return backward_t<float>(dy, z, x, ldx, w, M, K, N, act, dtype, 1, dx, dw, db, (char *)work, st);
   if (dtype == CINEMA_DT_BF16) return backward_t<bf16_t>(dy, z, x, ldx, w, M, K, N, act, dtype, db_f32, dx, dw, db, (char *)work, st);

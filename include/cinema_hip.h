@@ -518,7 +518,7 @@ int cinema_linear_forward(const void *x, int64_t ldx, const void *w, const void 
 /* dz = dy * act'(z);  dx [M x K] = dz W,  dw [N x K] = dz^T x,  db [N] = column sums of dz (fp32 if db_f32, else the rows'
  * type).  dx, dw, db may be NULL.  z may be NULL for CINEMA_ACT_NONE.  The residual's gradient is dy itself.  Every sum has a
  * fixed order: equal inputs give equal bits.  work: cinema_linear_work_bytes(..., 1) bytes, asked with the x, ldx and w given
- * here (NULL where NULL is given). */
+ * here (NULL where NULL is given); NULL if 0. */
 int cinema_linear_backward(const void *dy, const void *z, const void *x, int64_t ldx, const void *w, int64_t M, int64_t K,
                            int64_t N, int32_t act, int32_t dtype, int32_t db_f32, void *dx, void *dw, void *db, void *work,
                            void *stream);

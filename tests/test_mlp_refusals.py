@@ -93,7 +93,7 @@ def test_c_entry_points_check_their_arguments():
     a = list(ok)
     a[5], a[6] = one, 7
     assert lib.cinema_linear_forward(*a) != 0                                    # residual rows closer than a row
-    ok = [one, one, one, 8, one, 16, 8, 8, 1, dt, 0, one, one, one, one, None]
+    ok = [one, one, one, 8, one, 5000, 8, 8, 1, dt, 0, one, one, one, one, None]
     for at, v in [(0, None), (1, None), (2, None), (3, 7), (4, None), (8, 5), (9, 4), (14, None), (5, 0)]:
         a = list(ok)
         a[at] = v
