@@ -186,9 +186,9 @@ SIGNATURES["cinema_adamw_step_clear"] = [C.POINTER(AdamWGroup), _I32, _P]
 
 DT_F32, DT_BF16, DT_F16 = 0, 1, 2
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
-SIGNATURES["cinema_linear_work_bytes"] = [_P, _I64, _P, _I64, _I64, _I64, _I32, _I32]
-SIGNATURES["cinema_linear_forward"] = [_P, _I64, _P, _P, _I32, _P, _I64, _I64, _I64, _I64, _I32, _I32, _P, _P, _P, _P]
-SIGNATURES["cinema_linear_backward"] = [_P, _P, _P, _I64, _P, _I64, _I64, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P]
+SIGNATURES["cinema_linear_work_bytes"] = [_P, _I64, _P, _I64, _I64, _I64, _I32, _I32, _I32]
+SIGNATURES["cinema_linear_forward"] = [_P, _I64, _P, _P, _I32, _P, _I64, _I64, _I64, _I64, _I32, _I32, _P, _I32, _P, _P, _P]
+SIGNATURES["cinema_linear_backward"] = [_P, _P, _I32, _P, _I64, _P, _I64, _I64, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P]
 _RESTYPES["cinema_linear_work_bytes"] = C.c_int64
 SIGNATURES["cinema_layer_norm_work_bytes"] = [_I64, _I64, _I32]
 SIGNATURES["cinema_layer_norm_forward"] = [_P, _I64, _P, _P, _I32, _I64, _I64, _F, _I32, _P, _P, _P, _P]

@@ -140,8 +140,8 @@ struct LinearActBackward : public Node {
     const Tensor xs = x.unpack(), ws = w.unpack(), zs = z.unpack();
     const int dt = dtype_of(g.scalar_type());
     const void *xp = need_w ? data(xs) : nullptr, *wp = need_x ? data(ws) : nullptr;
-    const Tensor work = workspace(api.linear_work_bytes(xp, ldx, wp, m, k, n, dt, 1), "cinema_linear_work_bytes", g);
-    check(api.linear_backward(data(g), data(zs), xp, ldx, wp, m, k, n, act, dt,
+    const Tensor work = workspace(api.linear_work_bytes(xp, ldx, wp, m, k, n, act, dt, 1), "cinema_linear_work_bytes", g);
+    check(api.linear_backward(data(g), data(zs), zs.defined() && zs.scalar_type() == at::kFloat, xp, ldx, wp, m, k, n, act, dt,
                               bias_type == at::kFloat, out(got[0]), out(got[1]), out(got[2]), out(work), stream_of(g)),
           "cinema_linear_backward");
     return got;
@@ -193,16 +193,18 @@ Tensor linear_act(Tensor x, Tensor w, const MaybeTensor &bias, const MaybeTensor
     at::AutoDispatchBelowADInplaceOrView below;
     const c10::DeviceGuard guard(x.device());
     y = at::empty(y_shape, x.options());
-    if (inner && act != CINEMA_ACT_NONE) z = at::empty({m, n}, x.options().dtype(x.scalar_type() == at::kFloat ? at::kFloat : at::kHalf));
+    // 16-bit rows keep fp16 pre-activations; where few of them make a gradient their rounding would show, and fp32 costs nothing
+    if (inner && act != CINEMA_ACT_NONE)
+      z = at::empty({m, n}, x.options().dtype(x.scalar_type() == at::kFloat || m * n <= 1 << 18 || n * k <= 2048 ? at::kFloat : at::kHalf));
     xr = rows_of(x, k);
     wc = w.contiguous();
     if (b.defined()) bc = b.contiguous();
     if (r.defined()) rr = rows_of(r, n);
     if (m > 0) {
       const int dt = dtype_of(x.scalar_type());
-      const Tensor work = workspace(api.linear_work_bytes(data(xr.t), xr.ld, data(wc), m, k, n, dt, 0), "cinema_linear_work_bytes", x);
+      const Tensor work = workspace(api.linear_work_bytes(data(xr.t), xr.ld, data(wc), m, k, n, act, dt, 0), "cinema_linear_work_bytes", x);
       check(api.linear_forward(data(xr.t), xr.ld, data(wc), data(bc), bc.defined() && bc.scalar_type() == at::kFloat, data(rr.t), rr.ld, m, k, n,
-                               act, dt, out(z), out(y), out(work), stream_of(x)),
+                               act, dt, out(z), z.defined() && z.scalar_type() == at::kFloat, out(y), out(work), stream_of(x)),
             "cinema_linear_forward");
     }
   }

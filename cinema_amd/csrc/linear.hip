@@ -7,6 +7,7 @@
 #include "mlp_gemm.h"
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace {
 
@@ -162,6 +163,8 @@ struct Epilogue {
   float *part;           // split reduction: raw sums [split][I][ldp], the rest is done by k_linear_join
   int64_t ldres, ldp;
   int act, bias_f32;
+  int z_f32;             // z is fp32 whatever the rows' type
+  int out_dt;            // type of `out`; another than T's only where fp32 products serve 16-bit rows
 };
 
 template <typename T>
@@ -176,6 +179,15 @@ __device__ __forceinline__ void load_bias(const Epilogue &e, int64_t j, int n, f
   }
 }
 
+template <typename T>
+__device__ __forceinline__ void store_out8(const Epilogue &e, int64_t at, int n, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    if (e.out_dt == CINEMA_DT_BF16) { store8((bf16_t *)e.out + at, n, v); return; }
+    if (e.out_dt == CINEMA_DT_F16) { store8((f16_t *)e.out + at, n, v); return; }
+  }
+  store8((T *)e.out + at, n, v);
+}
+
 // eight sums of row i, columns j .. j + n - 1, the bias in them; r: the residual's values
 template <typename T>
 __device__ __forceinline__ void finish8(const Epilogue &e, int64_t i, int64_t j, int n, int64_t J, float (&v)[8], const float (&r)[8]) {
@@ -184,14 +196,15 @@ __device__ __forceinline__ void finish8(const Epilogue &e, int64_t i, int64_t j,
     float h[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) h[k] = kept_value(v[k], e.act);
-    store8((Z *)e.z + i * J + j, n, h);
+    if (e.z_f32) store8((float *)e.z + i * J + j, n, h);
+    else store8((Z *)e.z + i * J + j, n, h);
   }
   act_values<sizeof(T) == 2>(v, e.act);
   if (e.res != nullptr) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] += r[k];
   }
-  store8((T *)e.out + i * J + j, n, v);
+  store_out8<T>(e, i * J + j, n, v);
 }
 
 // The results leave through LDS (32 x BJ/WJ values per wave at a time): the matrix unit's layout puts a row's neighbours into
@@ -241,25 +254,28 @@ __device__ __forceinline__ void write_tile(const f32x16 (&acc)[G::TI][G::TJ], in
 #pragma unroll
       for (int k = 0; k < 4; ++k) { v[8 * p + k] = a[k]; v[8 * p + 4 + k] = b[k]; }
     }
-    auto store_all = [&](auto *out, int64_t ld, int width, auto value) {       // rows of `ld` values, `width` of them from column j on
+    auto store_all = [&](auto store, auto value) {          // store(row, values, eight values)
 #pragma unroll
       for (int p = 0; p < PASSES; ++p) {
         float o[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) o[k] = value(8 * p + k);
-        if (FULL || ix + p * RPP < I) store8(out + (ix + p * RPP) * ld + j, FULL ? 8 : width, o);
+        if (FULL || ix + p * RPP < I) store(ix + p * RPP, FULL ? 8 : n, o);
       }
     };
     if (e.part != nullptr) {
-      store_all(e.part, e.ldp, n > 0 ? 8 : 0, [&](int k) { return v[k]; });    // ldp is a multiple of 8
+      store_all([&](int64_t i, int w, const float(&o)[8]) { store8(e.part + i * e.ldp + j, w > 0 ? 8 : 0, o); },   // ldp is a multiple of 8
+                [&](int k) { return v[k]; });
     } else {
-      if (e.z != nullptr) store_all((typename Kept<T>::type *)e.z, J, n, [&](int k) { return kept_value(v[k], e.act); });
+      auto kept = [&](int k) { return kept_value(v[k], e.act); };
+      if (e.z != nullptr && e.z_f32) store_all([&](int64_t i, int w, const float(&o)[8]) { store8((float *)e.z + i * J + j, w, o); }, kept);
+      else if (e.z != nullptr) store_all([&](int64_t i, int w, const float(&o)[8]) { store8((typename Kept<T>::type *)e.z + i * J + j, w, o); }, kept);
       act_values<sizeof(T) == 2>(v, e.act);
       if (e.res != nullptr) {
 #pragma unroll
         for (int k = 0; k < PASSES * 8; ++k) v[k] += (float)res[k / 8][k % 8];
       }
-      store_all((T *)e.out, J, n, [&](int k) { return v[k]; });
+      store_all([&](int64_t i, int w, const float(&o)[8]) { store_out8<T>(e, i * J + j, w, o); }, [&](int k) { return v[k]; });
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -391,7 +407,8 @@ __global__ __launch_bounds__(256) void k_linear_rows(const T *x, int64_t ldx, co
   if (lane >= NV || m >= M || f0 + f >= N) return;
   const int64_t j = f0 + f, o = (m0 + m) * N + j;
   if (e.bias != nullptr) z += e.bias_f32 ? ((const float *)e.bias)[j] : (float)((const T *)e.bias)[j];
-  if (e.z != nullptr) ((Z *)e.z)[o] = (Z)kept_value(z, e.act);
+  if (e.z != nullptr && e.z_f32) ((float *)e.z)[o] = kept_value(z, e.act);
+  else if (e.z != nullptr) ((Z *)e.z)[o] = (Z)kept_value(z, e.act);
   float v[1] = {z};
   act_values<sizeof(T) == 2>(v, e.act);
   if (e.res != nullptr) v[0] += (float)((const T *)e.res)[(m0 + m) * e.ldres + j];
@@ -401,10 +418,10 @@ __global__ __launch_bounds__(256) void k_linear_rows(const T *x, int64_t ldx, co
 // dz = dy * act'(z) and the column sums of dz over the block's rows.  A workgroup takes 512 columns (64 lanes x 8) and `rows`
 // rows, its eight waves every eighth row, two of them under way; sums of the waves meet in LDS.  dz has rows of ldz values, zeros behind the N'th (the
 // products read whole chunks).  dz == null: only the sums.  Bound by memory: 25000 x 512 bf16, 77 MB, 18 us = 4.2 TB/s.
-template <typename T>
-__global__ __launch_bounds__(512) void k_linear_dz(const T *dy, const void *zv, T *dz, int64_t ldz, float *part, int64_t M, int64_t N, int64_t rows,
+template <typename T, typename TO, bool Z32>
+__global__ __launch_bounds__(512) void k_linear_dz(const T *dy, const void *zv, TO *dz, int64_t ldz, float *part, int64_t M, int64_t N, int64_t rows,
                                                    int act, void *db, int db_f32) {
-  typedef typename Kept<T>::type Z;
+  typedef std::conditional_t<Z32, float, typename Kept<T>::type> Z;
   __shared__ float red[8][512];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t j = (int64_t)blockIdx.x * 512 + lane * 8;
@@ -474,7 +491,7 @@ __global__ __launch_bounds__(512) void k_linear_dz(const T *dy, const void *zv, 
 // coef comes from dy and z into LDS (a broadcast per product); blockIdx.y counts the eights of dx, then those of dW.
 constexpr int SMALL_R = 512;
 template <typename T>
-__global__ __launch_bounds__(256) void k_linear_small(const T *dy, const void *zv, const T *x, int64_t ldx, const T *w, int M, int K, int N, int act,
+__global__ __launch_bounds__(256) void k_linear_small(const T *dy, const void *zv, const T *x, int64_t ldx, const T *w, int M, int K, int N, int act, int z_f32,
                                                       T *dx, T *dw, void *db, int db_f32) {
   typedef typename Kept<T>::type Z;
   __shared__ __attribute__((aligned(16))) float coef[SMALL_R][8];
@@ -490,7 +507,8 @@ __global__ __launch_bounds__(256) void k_linear_small(const T *dy, const void *z
     if (m < M && n < N) {
       g[0] = (float)dy[(int64_t)m * N + n];
       if (act != ACT_NONE) {
-        const float z[8] = {(float)((const Z *)zv)[(int64_t)m * N + n], 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        const int64_t at = (int64_t)m * N + n;
+        const float z[8] = {z_f32 ? ((const float *)zv)[at] : (float)((const Z *)zv)[at], 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         slope8<sizeof(T) == 2>(g, z, act);
       }
     }
@@ -557,18 +575,29 @@ __global__ __launch_bounds__(256) void k_linear_small(const T *dy, const void *z
 
 // 8191 x 257 fp16 with a weight of 1283 x 257: 5.4 us, mostly the trip to memory.
 // rows [R][ld] of C values -> [R][ldo], ldo the next multiple of a chunk, zeros behind; a thread moves a chunk.  Two at once.
+// TO: the same type, or fp32.
 struct Pack { const void *src; void *dst; int64_t rows, cols, ld, ldo; };
-template <typename T>
+template <typename T, typename TO>
 __global__ __launch_bounds__(256) void k_linear_pack(Pack a, Pack b) {
   const Pack p = blockIdx.y == 0 ? a : b;
-  constexpr int V = 16 / sizeof(T);
+  constexpr int V = 16 / sizeof(TO);
   const unsigned per = (unsigned)(p.ldo / V);
   const int64_t total = p.rows * per;
   for (int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x; g < total; g += (int64_t)gridDim.x * 256) {
     const int64_t row = total <= 0xffffffffll ? (int64_t)((unsigned)g / per) : g / per;
     const int64_t c = (g - row * per) * V;
-    const u32x4 v = load_chunk((const T *)p.src + row * p.ld + c, p.cols - c < V ? (int)(p.cols - c) : V);
-    *(u32x4 *)((T *)p.dst + row * p.ldo + c) = v;
+    const int n = p.cols - c < V ? (int)(p.cols - c) : V;
+    const T *src = (const T *)p.src + row * p.ld + c;
+    u32x4 v;
+    if constexpr (std::is_same_v<T, TO>) {
+      v = load_chunk(src, n);
+    } else {
+      TO e[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) e[k] = k < n ? (TO)src[k] : (TO)0.f;
+      __builtin_memcpy(&v, e, 16);
+    }
+    *(u32x4 *)((TO *)p.dst + row * p.ldo + c) = v;
   }
 }
 
@@ -667,31 +696,36 @@ bool whole_chunks(const void *p, int64_t ld, int64_t cols, int dt) {
   return ((uintptr_t)p & 15) == 0 && ld % v == 0 && cols % v == 0 && ld < (1 << 20);
 }
 int64_t padded(int64_t cols, int dt) { return up(cols, 16 / elem_size(dt)) * (16 / elem_size(dt)); }
-int64_t pack_bytes(const void *p, int64_t ld, int64_t rows, int64_t cols, int dt) {
+// wide: 16-bit rows as fp32, always packed
+int64_t pack_bytes(const void *p, int64_t ld, int64_t rows, int64_t cols, int dt, bool wide) {
+  if (wide) return align256(rows * padded(cols, CINEMA_DT_F32) * 4);
   return whole_chunks(p, ld, cols, dt) ? 0 : align256(rows * padded(cols, dt) * elem_size(dt));
 }
 
-// x [xr][xc] and w [wr][wc] as the products read them: in place, or packed to `at` (one launch for both)
-template <typename T>
+// x [xr][xc] and w [wr][wc] as the products read them: in place, or packed to `at` (one launch for both), as TO
+template <typename T, typename TO>
 int pack_operands(const void *&x, int64_t &ldx, int64_t xr, int64_t xc, const void *&w, int64_t &ldw, int64_t wr, int64_t wc, int dt, char *at,
                   hipStream_t st) {
+  constexpr bool wide = !std::is_same_v<T, TO>;
+  const int to = wide ? CINEMA_DT_F32 : dt;
   Pack p[2] = {};
   int n = 0;
-  if (x != nullptr && !whole_chunks(x, ldx, xc, dt)) {
-    p[n++] = {x, at, xr, xc, ldx, padded(xc, dt)};
-    at += align256(xr * padded(xc, dt) * (int64_t)sizeof(T));
+  if (x != nullptr && (wide || !whole_chunks(x, ldx, xc, dt))) {
+    p[n++] = {x, at, xr, xc, ldx, padded(xc, to)};
+    at += align256(xr * padded(xc, to) * (int64_t)sizeof(TO));
     x = p[n - 1].dst;
     ldx = p[n - 1].ldo;
   }
-  if (w != nullptr && !whole_chunks(w, ldw, wc, dt)) {
-    p[n++] = {w, at, wr, wc, ldw, padded(wc, dt)};
+  if (w != nullptr && (wide || !whole_chunks(w, ldw, wc, dt))) {
+    p[n++] = {w, at, wr, wc, ldw, padded(wc, to)};
     w = p[n - 1].dst;
     ldw = p[n - 1].ldo;
   }
   if (n == 0) return 0;
   int64_t most = 0;
-  for (int i = 0; i < n; ++i) most = std::max(most, p[i].rows * p[i].ldo / (16 / (int64_t)sizeof(T)));
-  hipLaunchKernelGGL(k_linear_pack<T>, dim3((unsigned)std::min<int64_t>(up(most, 256), 8 * cinema_cu_count()), n), dim3(256), 0, st, p[0], p[1]);
+  for (int i = 0; i < n; ++i) most = std::max(most, p[i].rows * p[i].ldo / (16 / (int64_t)sizeof(TO)));
+  auto fn = k_linear_pack<T, TO>;
+  hipLaunchKernelGGL(fn, dim3((unsigned)std::min<int64_t>(up(most, 256), 8 * cinema_cu_count()), n), dim3(256), 0, st, p[0], p[1]);
   CINEMA_CHECK_HIP(hipGetLastError());
   return 0;
 }
@@ -763,15 +797,23 @@ bool small_backward(int64_t M, int64_t K, int64_t N, int dt) {
   return std::max(M, N) <= (f32 ? SMALL_R : SMALL_R / 2) && M * K * N <= (f32 ? 32 << 20 : 17 << 20);
 }
 
+// dz of a smooth activation is rounded to 16 bits for the matrix unit.  Where few values of it (M N) or few sums over it (N K)
+// make the gradients, those roundings do not average out (971 x 1 x 3: dW off by 0.006 of its norm, 0.0017 is its own rounding),
+// and the products are small: they then run in fp32.
+bool wide_backward(int64_t M, int64_t K, int64_t N, int act, int dt) {
+  return dt != CINEMA_DT_F32 && act != ACT_NONE && act != ACT_RELU && (N * K <= 2048 || M * N <= 8192);
+}
+
 struct BackwardPlan { int64_t ldz, dz, db, pack, part, total; };
-BackwardPlan plan_backward(const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N, int dt) {
+BackwardPlan plan_backward(const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N, int dt, bool wide) {
   BackwardPlan b;
-  b.ldz = padded(N, dt);
+  const int to = wide ? CINEMA_DT_F32 : dt;
+  b.ldz = padded(N, to);
   b.dz = 0;
-  b.db = align256(M * b.ldz * elem_size(dt));
+  b.db = align256(M * b.ldz * elem_size(to));
   b.pack = b.db + align256(up(M, dz_rows(M, N)) * N * 4);
-  b.part = b.pack + pack_bytes(x, ldx, M, K, dt) + pack_bytes(w, K, N, K, dt);
-  b.total = b.part + std::max(plan_product(M, K, N, dt, EPI_SUMS).part_bytes, plan_product(N, K, M, dt, EPI_SUMS).part_bytes);
+  b.part = b.pack + pack_bytes(x, ldx, M, K, dt, wide) + pack_bytes(w, K, N, K, dt, wide);
+  b.total = b.part + std::max(plan_product(M, K, N, to, EPI_SUMS).part_bytes, plan_product(N, K, M, to, EPI_SUMS).part_bytes);
   return b;
 }
 int64_t forward_part_bytes(int64_t M, int64_t K, int64_t N, int dt) {       // whatever the epilogue will be
@@ -779,14 +821,14 @@ int64_t forward_part_bytes(int64_t M, int64_t K, int64_t N, int dt) {       // w
                    plan_product(M, N, K, dt, EPI_HEAVY).part_bytes});
 }
 int64_t forward_pack_bytes(const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N, int dt) {
-  return pack_bytes(x, ldx, M, K, dt) + pack_bytes(w, K, N, K, dt);
+  return pack_bytes(x, ldx, M, K, dt, false) + pack_bytes(w, K, N, K, dt, false);
 }
 
 template <typename T>
 int forward_t(const void *x, int64_t ldx, const void *w, const void *bias, int bias_f32, const void *res, int64_t ldres, int64_t M, int64_t K,
-              int64_t N, int act, int dt, void *z, void *y, char *work, hipStream_t st) {
+              int64_t N, int act, int dt, void *z, int z_f32, void *y, char *work, hipStream_t st) {
   Epilogue e = {};
-  e.bias = bias; e.bias_f32 = bias_f32; e.res = res; e.ldres = ldres; e.act = act; e.z = z; e.out = y;
+  e.z_f32 = z_f32; e.out_dt = dt; e.bias = bias; e.bias_f32 = bias_f32; e.res = res; e.ldres = ldres; e.act = act; e.z = z; e.out = y;
   if (by_rows(M, K, N, dt)) {
     if (M == 1) hipLaunchKernelGGL((k_linear_rows<T, 1, 2>), dim3((unsigned)up(N, 8)), dim3(256), 0, st, (const T *)x, ldx, (const T *)w, (int)M, K, N, e);
     else if (M <= 4) hipLaunchKernelGGL((k_linear_rows<T, 4, 4>), dim3((unsigned)up(N, 16)), dim3(256), 0, st, (const T *)x, ldx, (const T *)w, (int)M, K, N, e);
@@ -796,92 +838,110 @@ int forward_t(const void *x, int64_t ldx, const void *w, const void *bias, int b
   }
   char *part = work + forward_pack_bytes(x, ldx, w, M, K, N, dt);
   int64_t ldw = K;
-  const int rc = pack_operands<T>(x, ldx, M, K, w, ldw, N, K, dt, work, st);
+  const int rc = pack_operands<T, T>(x, ldx, M, K, w, ldw, N, K, dt, work, st);
   if (rc != 0) return rc;
   const GemmOperand A = {x, ldx, M, K}, B = {w, ldw, N, K};
   return product<T, false, false>(A, B, e, dt, part, st);
 }
 
-template <typename T>
-int backward_t(const void *dy, const void *z, const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N, int act, int dt,
-               int db_f32, void *dx, void *dw, void *db, char *work, hipStream_t st) {
-  if (small_backward(M, K, N, dt)) {
-    const unsigned blocks = (unsigned)((dx != nullptr ? up(M, 8) : 0) + (dw != nullptr || db != nullptr ? up(N, 8) : 0));
-    if (blocks == 0) return 0;
-    hipLaunchKernelGGL(k_linear_small<T>, dim3((unsigned)up(K, 64), blocks), dim3(256), 0, st, (const T *)dy, z, (const T *)x, ldx, (const T *)w,
-                       (int)M, (int)K, (int)N, act, (T *)dx, (T *)dw, db, db_f32);
+template <typename T, typename TO>
+int launch_dz(const void *dy, const void *z, int z_f32, void *dz, int64_t ldz, float *part, int64_t M, int64_t N, int act, void *db, int db_f32,
+              hipStream_t st) {
+  const int64_t rows = dz_rows(M, N), P = up(M, rows);
+  auto fn = z_f32 ? k_linear_dz<T, TO, true> : k_linear_dz<T, TO, false>;
+  hipLaunchKernelGGL(fn, dim3((unsigned)up(N, 512), (unsigned)P), dim3(512), 0, st, (const T *)dy, z, (TO *)dz, ldz, part, M, N, rows, act, db, db_f32);
+  CINEMA_CHECK_HIP(hipGetLastError());
+  if (db != nullptr && P > 1) {
+    hipLaunchKernelGGL(k_column_join<T>, dim3((unsigned)up(N, 32)), dim3(1024), 0, st, part, (int)P, N, db, db_f32);
     CINEMA_CHECK_HIP(hipGetLastError());
-    return 0;
   }
-  const BackwardPlan bp = plan_backward(x, ldx, w, M, K, N, dt);
+  return 0;
+}
+
+// TO: the type that dz is kept and the products run in, T's or fp32
+template <typename T, typename TO>
+int backward_t(const void *dy, const void *z, int z_f32, const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N, int act, int dt,
+               int db_f32, void *dx, void *dw, void *db, char *work, hipStream_t st) {
+  constexpr bool wide = !std::is_same_v<T, TO>;
+  const int to = wide ? CINEMA_DT_F32 : dt;
+  const BackwardPlan bp = plan_backward(x, ldx, w, M, K, N, dt, wide);
   const void *dz = dy;
   int64_t ldz = N;
-  const bool rewrite = (dx != nullptr || dw != nullptr) && (act != ACT_NONE || !whole_chunks(dy, N, N, dt));
+  const bool products = dx != nullptr || dw != nullptr;
+  const bool rewrite = act != ACT_NONE || (products && !whole_chunks(dy, N, N, dt));      // db alone needs the slope too
   if (rewrite || db != nullptr) {
-    const int64_t rows = dz_rows(M, N), P = up(M, rows);
-    T *out = rewrite ? (T *)(work + bp.dz) : nullptr;
-    float *part = db != nullptr ? (float *)(work + bp.db) : nullptr;
-    // db alone of an activation: its sums need the slope, so dz is written all the same
-    if (db != nullptr && act != ACT_NONE) out = (T *)(work + bp.dz);
-    hipLaunchKernelGGL(k_linear_dz<T>, dim3((unsigned)up(N, 512), (unsigned)P), dim3(512), 0, st, (const T *)dy, z, out, bp.ldz, part, M, N, rows, act,
-                       db, db_f32);
-    CINEMA_CHECK_HIP(hipGetLastError());
-    if (out != nullptr) { dz = out; ldz = bp.ldz; }
-    if (db != nullptr && P > 1) {
-      hipLaunchKernelGGL(k_column_join<T>, dim3((unsigned)up(N, 32)), dim3(1024), 0, st, part, (int)P, N, db, db_f32);
-      CINEMA_CHECK_HIP(hipGetLastError());
-    }
+    const int rc = launch_dz<T, TO>(dy, z, z_f32, rewrite ? work + bp.dz : nullptr, bp.ldz, db != nullptr ? (float *)(work + bp.db) : nullptr, M, N, act,
+                                    db, db_f32, st);
+    if (rc != 0) return rc;
+    if (rewrite) { dz = work + bp.dz; ldz = bp.ldz; }
   }
   int64_t ldw = K;
   if (dx == nullptr) w = nullptr;
   if (dw == nullptr) x = nullptr;
-  int rc = pack_operands<T>(x, ldx, M, K, w, ldw, N, K, dt, work + bp.pack, st);
+  int rc = pack_operands<T, TO>(x, ldx, M, K, w, ldw, N, K, dt, work + bp.pack, st);
   if (rc != 0) return rc;
   Epilogue e = {};
+  e.out_dt = dt;
   if (dx != nullptr) {
     e.out = dx;
     const GemmOperand A = {dz, ldz, M, N}, B = {w, ldw, K, N};
-    rc = product<T, false, true>(A, B, e, dt, work + bp.part, st);
+    rc = product<TO, false, true>(A, B, e, to, work + bp.part, st);
     if (rc != 0) return rc;
   }
   if (dw != nullptr) {
     e.out = dw;
     const GemmOperand A = {dz, ldz, N, M}, B = {x, ldx, K, M};
-    rc = product<T, true, true>(A, B, e, dt, work + bp.part, st);
+    rc = product<TO, true, true>(A, B, e, to, work + bp.part, st);
     if (rc != 0) return rc;
   }
   return 0;
 }
 
+template <typename T>
+int backward_any(const void *dy, const void *z, int z_f32, const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N, int act, int dt,
+                 int db_f32, void *dx, void *dw, void *db, char *work, hipStream_t st) {
+  if (small_backward(M, K, N, dt)) {
+    const unsigned blocks = (unsigned)((dx != nullptr ? up(M, 8) : 0) + (dw != nullptr || db != nullptr ? up(N, 8) : 0));
+    if (blocks == 0) return 0;
+    hipLaunchKernelGGL(k_linear_small<T>, dim3((unsigned)up(K, 64), blocks), dim3(256), 0, st, (const T *)dy, z, (const T *)x, ldx, (const T *)w,
+                       (int)M, (int)K, (int)N, act, z_f32, (T *)dx, (T *)dw, db, db_f32);
+    CINEMA_CHECK_HIP(hipGetLastError());
+    return 0;
+  }
+  if (wide_backward(M, K, N, act, dt)) return backward_t<T, float>(dy, z, z_f32, x, ldx, w, M, K, N, act, dt, db_f32, dx, dw, db, work, st);
+  return backward_t<T, T>(dy, z, z_f32, x, ldx, w, M, K, N, act, dt, db_f32, dx, dw, db, work, st);
+}
+
 }  // namespace
 
-extern "C" int64_t cinema_linear_work_bytes(const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N, int32_t dtype,
+extern "C" int64_t cinema_linear_work_bytes(const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N, int32_t act, int32_t dtype,
                                             int32_t backward) {
   if (check_sizes("cinema_linear_work_bytes", M, K, N, dtype) != 0) return -1;
-  if (backward) return small_backward(M, K, N, dtype) ? 0 : plan_backward(x, ldx, w, M, K, N, dtype).total;
+  if (backward) return small_backward(M, K, N, dtype) ? 0 : plan_backward(x, ldx, w, M, K, N, dtype, wide_backward(M, K, N, act, dtype)).total;
   return by_rows(M, K, N, dtype) ? 0 : forward_pack_bytes(x, ldx, w, M, K, N, dtype) + forward_part_bytes(M, K, N, dtype);
 }
 
 extern "C" int cinema_linear_forward(const void *x, int64_t ldx, const void *w, const void *bias, int32_t bias_f32, const void *res, int64_t ldres,
-                                     int64_t M, int64_t K, int64_t N, int32_t act, int32_t dtype, void *z, void *y, void *work, void *stream) {
+                                     int64_t M, int64_t K, int64_t N, int32_t act, int32_t dtype, void *z, int32_t z_f32, void *y, void *work,
+                                     void *stream) {
   if (check_sizes("cinema_linear_forward", M, K, N, dtype) != 0) return -1;
   CINEMA_REQUIRE(x && w && y && ldx >= K && (!res || ldres >= N), "cinema_linear_forward: null operand, or a row stride below the row");
   CINEMA_REQUIRE(act >= 0 && act < ACT_COUNT, "cinema_linear_forward: unknown activation %d", act);
-  CINEMA_REQUIRE(work || cinema_linear_work_bytes(x, ldx, w, M, K, N, dtype, 0) == 0, "cinema_linear_forward: null workspace");
+  CINEMA_REQUIRE(work || cinema_linear_work_bytes(x, ldx, w, M, K, N, act, dtype, 0) == 0, "cinema_linear_forward: null workspace");
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == CINEMA_DT_F32) return forward_t<float>(x, ldx, w, bias, 1, res, ldres, M, K, N, act, dtype, z, y, (char *)work, st);
-  if (dtype == CINEMA_DT_BF16) return forward_t<bf16_t>(x, ldx, w, bias, bias_f32, res, ldres, M, K, N, act, dtype, z, y, (char *)work, st);
-  return forward_t<f16_t>(x, ldx, w, bias, bias_f32, res, ldres, M, K, N, act, dtype, z, y, (char *)work, st);
+  if (dtype == CINEMA_DT_F32) return forward_t<float>(x, ldx, w, bias, 1, res, ldres, M, K, N, act, dtype, z, z_f32, y, (char *)work, st);
+  if (dtype == CINEMA_DT_BF16) return forward_t<bf16_t>(x, ldx, w, bias, bias_f32, res, ldres, M, K, N, act, dtype, z, z_f32, y, (char *)work, st);
+  return forward_t<f16_t>(x, ldx, w, bias, bias_f32, res, ldres, M, K, N, act, dtype, z, z_f32, y, (char *)work, st);
 }
 
-extern "C" int cinema_linear_backward(const void *dy, const void *z, const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N,
+extern "C" int cinema_linear_backward(const void *dy, const void *z, int32_t z_f32, const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N,
                                       int32_t act, int32_t dtype, int32_t db_f32, void *dx, void *dw, void *db, void *work, void *stream) {
   if (check_sizes("cinema_linear_backward", M, K, N, dtype) != 0) return -1;
   CINEMA_REQUIRE(act >= 0 && act < ACT_COUNT, "cinema_linear_backward: unknown activation %d", act);
   CINEMA_REQUIRE(dy && (act == ACT_NONE || z) && (!dx || w) && (!dw || x) && (!dw || ldx >= K), "cinema_linear_backward: null operand, or a row stride below the row");
-  CINEMA_REQUIRE(work || cinema_linear_work_bytes(x, ldx, w, M, K, N, dtype, 1) == 0, "cinema_linear_backward: null workspace");
+  CINEMA_REQUIRE(work || cinema_linear_work_bytes(x, ldx, w, M, K, N, act, dtype, 1) == 0, "cinema_linear_backward: null workspace");
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == CINEMA_DT_F32) return backward_t<float>(dy, z, x, ldx, w, M, K, N, act, dtype, 1, dx, dw, db, (char *)work, st);
-  if (dtype == CINEMA_DT_BF16) return backward_t<bf16_t>(dy, z, x, ldx, w, M, K, N, act, dtype, db_f32, dx, dw, db, (char *)work, st);
-  return backward_t<f16_t>(dy, z, x, ldx, w, M, K, N, act, dtype, db_f32, dx, dw, db, (char *)work, st);
+  if (dtype == CINEMA_DT_F32) return backward_any<float>(dy, z, z_f32, x, ldx, w, M, K, N, act, dtype, 1, dx, dw, db, (char *)work, st);
+  if (dtype == CINEMA_DT_BF16) return backward_any<bf16_t>(dy, z, z_f32, x, ldx, w, M, K, N, act, dtype, db_f32, dx, dw, db, (char *)work, st);
+  return backward_any<f16_t>(dy, z, z_f32, x, ldx, w, M, K, N, act, dtype, db_f32, dx, dw, db, (char *)work, st);
 }

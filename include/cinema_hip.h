@@ -507,19 +507,19 @@ int cinema_adamw_step_clear(const cinema_adamw_group *groups /* host */, int32_t
 
 /* y [M x N] = act(x [M x K, row stride ldx] W [N x K]^T + bias [N]) + res [M x N, row stride ldres]; bias and res may be NULL.
  * bias is fp32 (bias_f32 != 0) or of the rows' type.  z (NULL if no gradient is wanted): what the backward pass reads of the
- * pre-activations, [M x N] fp16 for the 16-bit types, fp32 for fp32.  work: cinema_linear_work_bytes(..., 0) bytes (NULL if 0).
+ * pre-activations, [M x N] fp32 for fp32 rows or with z_f32 != 0, fp16 for the 16-bit types otherwise.  work: cinema_linear_work_bytes(..., 0) bytes (NULL if 0).
  * 1 <= M < 2^31, 1 <= K, N < 2^20; cinema_linear_work_bytes returns -1 for anything else.  It takes the x, ldx and w of the
  * call for their alignment: operands whose rows are not whole 16-byte pieces are packed into the workspace. */
-int64_t cinema_linear_work_bytes(const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N, int32_t dtype,
-                                 int32_t backward);
+int64_t cinema_linear_work_bytes(const void *x, int64_t ldx, const void *w, int64_t M, int64_t K, int64_t N, int32_t act,
+                                 int32_t dtype, int32_t backward);
 int cinema_linear_forward(const void *x, int64_t ldx, const void *w, const void *bias, int32_t bias_f32, const void *res,
-                          int64_t ldres, int64_t M, int64_t K, int64_t N, int32_t act, int32_t dtype, void *z, void *y,
-                          void *work, void *stream);
+                          int64_t ldres, int64_t M, int64_t K, int64_t N, int32_t act, int32_t dtype, void *z,
+                          int32_t z_f32, void *y, void *work, void *stream);
 /* dz = dy * act'(z);  dx [M x K] = dz W,  dw [N x K] = dz^T x,  db [N] = column sums of dz (fp32 if db_f32, else the rows'
- * type).  dx, dw, db may be NULL.  z may be NULL for CINEMA_ACT_NONE.  The residual's gradient is dy itself.  Every sum has a
+ * type).  dx, dw, db may be NULL.  z may be NULL for CINEMA_ACT_NONE (z_f32: as it was given to the forward pass).  The residual's gradient is dy itself.  Every sum has a
  * fixed order: equal inputs give equal bits.  work: cinema_linear_work_bytes(..., 1) bytes, asked with the x, ldx and w given
  * here (NULL where NULL is given); NULL if 0. */
-int cinema_linear_backward(const void *dy, const void *z, const void *x, int64_t ldx, const void *w, int64_t M, int64_t K,
+int cinema_linear_backward(const void *dy, const void *z, int32_t z_f32, const void *x, int64_t ldx, const void *w, int64_t M, int64_t K,
                            int64_t N, int32_t act, int32_t dtype, int32_t db_f32, void *dx, void *dw, void *db, void *work,
                            void *stream);
 

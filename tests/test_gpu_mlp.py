@@ -785,3 +785,22 @@ def test_linear_largest_tiles(dtype):
 def test_linear_largest_tiles_fp32():
     check_linear(16380, 2050, 1030, torch.float32, "silu")
     check_linear(16384, 2048, 1024, torch.float32, "gelu")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("m,k,n", [(971, 1, 3), (1, 700, 300), (5, 7, 900), (20000, 3, 2), (300, 2, 500), (17, 33, 20), (2, 64, 1000)])
+def test_linear_gradients_of_few_values_are_rounded_once(m, k, n, act, dtype):
+    """few values of dz, or few sums over it: nothing averages a rounding of dz out, so it stays in 32 bits.  Each gradient is
+    then its own value rounded (half a step U at most) plus sums in fp32 and the activation's 2^-21 -- which cancellation among
+    the terms magnifies, so they are taken relative to the sums of magnitudes"""
+    from cinema_amd.models.mlp import linear_act
+    x, w, b, _, dy = linear_data(m, k, n, dtype, seed=m + k + n, res=False)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    got = torch.autograd.grad(linear_act(*leaves, None, act), leaves, dy)
+    z = x.double() @ w.double().t() + b.double()
+    dz = dy.double() * slope64(z, act)
+    e = dy.double().abs() * ((z.abs() + 4) ** 2 * 2.0 ** -21 + CURV * (k + 2) * 2.0 ** -23 * (x.double().abs() @ w.double().abs().t() + b.double().abs()))
+    for g, v, err in ((got[0], dz @ w.double(), e @ w.double().abs()), (got[1], dz.t() @ x.double(), e.t() @ x.double().abs()), (got[2], dz.sum(0), e.sum(0))):
+        sums = (max(m, n) + 2) * 2.0 ** -23 * (err / e.max().clamp_min(1e-30) * dz.abs().max())
+        within(g, v, v.abs() * U[dtype] * 1.01 + 1.01 * (err + sums) + TINY[dtype], f"{m}x{k}x{n} {act}")

@@ -76,25 +76,25 @@ def test_c_entry_points_check_their_arguments():
     lib = _lib.load()
     dt = _lib.DT_BF16
     x = C.c_void_p(1 << 20)
-    assert lib.cinema_linear_work_bytes(x, 512, x, 25000, 512, 512, dt, 0) == 0
-    assert lib.cinema_linear_work_bytes(x, 512, x, 25000, 512, 512, dt, 1) >= 25000 * 512 * 2
-    assert lib.cinema_linear_work_bytes(x, 511, x, 25000, 511, 512, dt, 0) >= 25000 * 512 * 2        # packed rows
-    assert lib.cinema_linear_work_bytes(C.c_void_p((1 << 20) + 2), 512, x, 25000, 512, 512, dt, 0) >= 25000 * 512 * 2
+    assert lib.cinema_linear_work_bytes(x, 512, x, 25000, 512, 512, 2, dt, 0) == 0
+    assert lib.cinema_linear_work_bytes(x, 512, x, 25000, 512, 512, 2, dt, 1) >= 25000 * 512 * 2
+    assert lib.cinema_linear_work_bytes(x, 511, x, 25000, 511, 512, 2, dt, 0) >= 25000 * 512 * 2        # packed rows
+    assert lib.cinema_linear_work_bytes(C.c_void_p((1 << 20) + 2), 512, x, 25000, 512, 512, 2, dt, 0) >= 25000 * 512 * 2
     for bad in [(0, 8, 8, dt), (8, 0, 8, dt), (8, 8, -1, dt), (8, 8, 8, 3), (1 << 31, 8, 8, dt), (8, 1 << 20, 8, dt), (1 << 30, 8, 1 << 19, dt)]:
         for back in (0, 1):
-            assert lib.cinema_linear_work_bytes(x, 8, x, *bad, back) == -1
+            assert lib.cinema_linear_work_bytes(x, 8, x, *bad[:3], 2, bad[3], back) == -1
         assert b"cinema_linear" in lib.cinema_last_error()
     one = C.c_void_p(256)
-    ok = [one, 8, one, None, 0, None, 0, 16, 8, 8, 0, dt, None, one, None, None]
-    for at, v in [(0, None), (1, 7), (2, None), (10, 5), (10, -1), (11, 9), (13, None), (7, 0)]:
+    ok = [one, 8, one, None, 0, None, 0, 16, 8, 8, 0, dt, None, 0, one, None, None]
+    for at, v in [(0, None), (1, 7), (2, None), (10, 5), (10, -1), (11, 9), (14, None), (7, 0)]:
         a = list(ok)
         a[at] = v
         assert lib.cinema_linear_forward(*a) != 0
     a = list(ok)
     a[5], a[6] = one, 7
     assert lib.cinema_linear_forward(*a) != 0                                    # residual rows closer than a row
-    ok = [one, one, one, 8, one, 5000, 8, 8, 1, dt, 0, one, one, one, one, None]
-    for at, v in [(0, None), (1, None), (2, None), (3, 7), (4, None), (8, 5), (9, 4), (14, None), (5, 0)]:
+    ok = [one, one, 0, one, 8, one, 5000, 8, 8, 1, dt, 0, one, one, one, one, None]
+    for at, v in [(0, None), (1, None), (3, None), (4, 7), (5, None), (9, 5), (10, 4), (15, None), (6, 0)]:
         a = list(ok)
         a[at] = v
         assert lib.cinema_linear_backward(*a) != 0
