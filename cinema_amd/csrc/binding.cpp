@@ -9,6 +9,7 @@
 #include <ATen/autocast_mode.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <dlfcn.h>
 #include <algorithm>
@@ -113,6 +114,19 @@ void first_order_only(const char *what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), "cinema_amd ", what, ": the gradients have no second derivative (create_graph=True)");
 }
 
+// A leaf's accumulator node runs on the stream it was made on and lives as long as an eager graph that uses the leaf.  One of
+// the default stream cannot take part in a capture: the captured backward pass would end the process from the engine's thread.
+void check_capture(const char *what, std::initializer_list<const Tensor *> inputs) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  for (const Tensor *t : inputs) {
+    if (!wants_grad(*t) || t->grad_fn()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = node ? node->stream() : std::nullopt;
+    TORCH_CHECK(!stream || stream->id() != 0, "cinema_amd ", what, ": captured with gradients while an eager graph of the default stream ",
+                "uses the same leaves; release its results first, or capture under torch.no_grad()");
+  }
+}
+
 // ---- linear_act ------------------------------------------------------------------------------------------------------------
 struct LinearActBackward : public Node {
   SavedVariable x, w, z;
@@ -186,6 +200,7 @@ Tensor linear_act(Tensor x, Tensor w, const MaybeTensor &bias, const MaybeTensor
                     at::IntArrayRef(y_shape));
   check_gpu(what, x);
   const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || wants_grad(b) || wants_grad(r));
+  if (grad) check_capture(what, {&x, &w, &b, &r});
   const bool inner = grad && (x.requires_grad() || w.requires_grad() || wants_grad(b));      // something besides the residual
   Tensor y, z, wc, bc;
   Rows xr, rr;
@@ -287,6 +302,7 @@ Tensor layer_norm(Tensor x, const MaybeTensor &weight, const MaybeTensor &bias, 
   TORCH_CHECK_VALUE(eps >= 0, what, ": eps = ", eps);
   check_gpu(what, x);
   const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(w) || wants_grad(b));
+  if (grad) check_capture(what, {&x, &w, &b});
   const at::ScalarType w_type = w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : x.scalar_type();
   Tensor y, stats, wc, bc;
   Rows xr;

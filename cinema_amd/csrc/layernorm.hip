@@ -26,7 +26,7 @@ __device__ __forceinline__ float row_sum(float x, float *red, int slot) {
 // NW == 1: a workgroup of four waves, each with its own rows; else a workgroup of NW waves on one row after the other.  Weights
 // stay in registers over the rows (read per row they would be as many bytes from the L2 as the rows from memory), and the
 // next row is under way while this one is reduced.  bf16: 16384 x 4096 64 us = 4.2 TB/s (94 with weights read per row), 25000 x 512
-// 12 us = 4.3 TB/s.  
+// 12 us = 4.3 TB/s.
 template <typename T, typename W, int NW, int CH>
 __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void k_norm_fwd(const T *x, int64_t ldx, const W *w, const W *b, int64_t M, int D, float eps,
                                                                       T *y, float *mean, float *rstd) {

@@ -595,6 +595,43 @@ def test_operators_are_reproducible_and_replay_in_a_graph():
         assert all(torch.equal(p, q) for p, q in zip(got, want)), i
 
 
+@pytest.mark.parametrize("op", ["linear_act", "layer_norm"])
+def test_capture_beside_a_living_eager_graph_is_refused(op):
+    """a leaf whose accumulator belongs to the default stream cannot be captured with its gradients; without them it can"""
+    from cinema_amd.models.mlp import layer_norm, linear_act
+    x = torch.randn(40, 64, device="cuda")
+    w = torch.randn(64, 64, device="cuda") if op == "linear_act" else torch.randn(64, device="cuda")
+    w.requires_grad_(True)
+    call = linear_act if op == "linear_act" else layer_norm
+    eager = call(x, w)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            call(x, w)
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        y = call(x, w)
+    graph.replay()
+    assert torch.equal(y, eager)
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = call(x, w)
+        (dw,) = torch.autograd.grad(y, w, torch.ones_like(y))
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        v = call(x, w)
+        assert torch.equal(y, v) and torch.equal(dw, torch.autograd.grad(v, w, torch.ones_like(v))[0])
+        del v
+
+
+@pytest.mark.parametrize("m,k,n", [(4099, 257, 3), (33001, 33, 4), (300001, 5, 1), (1030, 1024, 2)])
+@pytest.mark.parametrize("act", ["none", "relu", "silu"])
+def test_linear_few_features_of_many_rows(m, k, n, act):
+    check_linear(m, k, n, torch.float32, act)
+
+
 def test_two_streams_at_once():
     """calls on two streams share nothing"""
     from cinema_amd.models.mlp import linear_act
