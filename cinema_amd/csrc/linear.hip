@@ -2,8 +2,10 @@
 //   z = x W^T + b,  y = act(z) + r;     dz = dy * act'(z),  dx = dz W,  dW = dz^T x,  db = sum over rows of dz
 // x [M][K], W [N][K], y [M][N] in fp32, bf16 or fp16; every sum and the whole epilogue in fp32, y, dx and dW rounded once.
 // 16-bit types keep z in fp16 (11 bits; act' of a bf16 z would add as much error as the rounding of the gradient itself, and
-// beyond 65504 act' does not change, so the range is enough), fp32 keeps it as it is.  dz is rounded to the matrix
-// instruction's input type: with 16-bit inputs there is no other way to feed it; db is summed before that rounding.
+// beyond 65504 act' does not change, so the range is enough) where z is large, in fp32 where it is small; fp32 keeps it as it is.
+// Large 16-bit products take dz rounded to the matrix instruction's input type, whose errors average out over the sums; where few
+// values or few sums make a gradient they do not, and dz stays in 32 bits there (small_backward and wide_backward).  db is
+// summed before the rounding.
 #include "mlp_gemm.h"
 #include <algorithm>
 #include <cmath>
@@ -345,17 +347,18 @@ __global__ __launch_bounds__(256) void k_linear_join(Epilogue e, int64_t I, int6
 
 // Few rows: bound by reading W once.  A wave owns FPW rows of W (output features) and MR rows of x at a time, its lanes share the
 // reduction 16 bytes at a time; x comes from the cache.  Small products of more rows too, blockIdx.y counting groups of MR: their
-// time is that of one trip to memory, which the tiles make twice (64 x 256 x 64 fp32: 7.5 us in a tile).
-template <typename T, int MR, int FPW>
+// time is that of one trip to memory, which the tiles make twice (64 x 256 x 64 fp32: 7.5 us in a tile).  NARROW: FPW features
+// at most, the waves count groups of rows.
+template <typename T, int MR, int FPW, bool NARROW>
 __global__ __launch_bounds__(256) void k_linear_rows(const T *x, int64_t ldx, const T *w, int M, int64_t K, int64_t N, Epilogue e) {
   constexpr int V = 16 / sizeof(T);
   typedef typename Kept<T>::type Z;
   const int lane = threadIdx.x & 63;
-  const int64_t m0 = (int64_t)blockIdx.y * MR;
+  const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t m0 = (NARROW ? wave : (int64_t)blockIdx.y) * MR, f0 = NARROW ? 0 : wave * FPW;
+  if (f0 >= N || m0 >= M) return;
   x += m0 * ldx;
   M -= (int)m0;
-  const int64_t f0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * FPW;
-  if (f0 >= N) return;
   float s[FPW][MR];
 #pragma unroll
   for (int f = 0; f < FPW; ++f)
@@ -634,8 +637,15 @@ struct Plan { int tile, splits; bool deep; int64_t per_split, ti, tj, ldp, part_
 // Rows against tiles in us: fp32 64 x 256 x 64 3.1 and 7.5, 1000 x 256 x 64 4.4 and 7.8, 512 x 512 x 512 14 and 11; bf16 (whose
 // tiles are faster, and whose short rows leave lanes idle) 64 x 1024 x 512 4.8 and 7.2, 256 x 256 x 256 4.8 and 4.2, 64 x 64 x 32
 // 4.5 and 3.2; with packing saved on top 256 x 257 x 129 5.0 and 11 (fp32), 5.8 and 7.6 (bf16).
+// Few features over many fp32 values of x, bound by reading x (a tile of 64 features reads it no faster and multiplies by
+// zeros): 65536 x 1024 -> 1 44 and 67 (6.0 TB/s, x partly in the cache), 53727 x 484 -> 3 17 and 38, 65536 x 33 -> 2 9.3 and 16,
+// 100000 x 64 -> 4 11.5 and 13.2, 20000 x 256 -> 1 4.2 and 4.0; 8 features 71 and 70.  bf16 tiles are as fast (65536 x 1024 -> 1
+// 22 and 22) or faster (100000 x 64 -> 4 15 and 7).
+bool narrow(int64_t M, int64_t K, int64_t N, int dt) {
+  return dt == CINEMA_DT_F32 && M > 8 && N <= 4 && M * K > (1 << 20) && up(M, 16) < (1 << 24);
+}
 bool by_rows(int64_t M, int64_t K, int64_t N, int dt) {
-  if (M <= 8) return true;
+  if (M <= 8 || narrow(M, K, N, dt)) return true;
   const bool f32 = dt == CINEMA_DT_F32, ragged = K % (16 / elem_size(dt)) != 0;
   return up(M, 8) * up(N, 2) <= (f32 || ragged ? 4096 : 2048) && K * elem_size(dt) <= 4096 && (f32 || K >= 256);
 }
@@ -829,10 +839,17 @@ int forward_t(const void *x, int64_t ldx, const void *w, const void *bias, int b
               int64_t N, int act, int dt, void *z, int z_f32, void *y, char *work, hipStream_t st) {
   Epilogue e = {};
   e.z_f32 = z_f32; e.out_dt = dt; e.bias = bias; e.bias_f32 = bias_f32; e.res = res; e.ldres = ldres; e.act = act; e.z = z; e.out = y;
+  if constexpr (std::is_same<T, float>::value) {
+    if (narrow(M, K, N, dt)) {
+      hipLaunchKernelGGL((k_linear_rows<T, 4, 4, true>), dim3((unsigned)up(M, 16)), dim3(256), 0, st, (const T *)x, ldx, (const T *)w, (int)M, K, N, e);
+      CINEMA_CHECK_HIP(hipGetLastError());
+      return 0;
+    }
+  }
   if (by_rows(M, K, N, dt)) {
-    if (M == 1) hipLaunchKernelGGL((k_linear_rows<T, 1, 2>), dim3((unsigned)up(N, 8)), dim3(256), 0, st, (const T *)x, ldx, (const T *)w, (int)M, K, N, e);
-    else if (M <= 4) hipLaunchKernelGGL((k_linear_rows<T, 4, 4>), dim3((unsigned)up(N, 16)), dim3(256), 0, st, (const T *)x, ldx, (const T *)w, (int)M, K, N, e);
-    else hipLaunchKernelGGL((k_linear_rows<T, 8, 2>), dim3((unsigned)up(N, 8), (unsigned)up(M, 8)), dim3(256), 0, st, (const T *)x, ldx, (const T *)w, (int)M, K, N, e);
+    if (M == 1) hipLaunchKernelGGL((k_linear_rows<T, 1, 2, false>), dim3((unsigned)up(N, 8)), dim3(256), 0, st, (const T *)x, ldx, (const T *)w, (int)M, K, N, e);
+    else if (M <= 4) hipLaunchKernelGGL((k_linear_rows<T, 4, 4, false>), dim3((unsigned)up(N, 16)), dim3(256), 0, st, (const T *)x, ldx, (const T *)w, (int)M, K, N, e);
+    else hipLaunchKernelGGL((k_linear_rows<T, 8, 2, false>), dim3((unsigned)up(N, 8), (unsigned)up(M, 8)), dim3(256), 0, st, (const T *)x, ldx, (const T *)w, (int)M, K, N, e);
     CINEMA_CHECK_HIP(hipGetLastError());
     return 0;
   }
