@@ -57,6 +57,12 @@ class HipAdamW(torch.optim.Optimizer):
     def step(self, closure=None, grad_norm=None):
         """grad_norm: with max_grad_norm, the norm to clip by (0-d fp32 device tensor) in place of this optimiser's own
         gradients' -- for a step whose gradients are spread over several optimisers or processes."""
+        if grad_norm is not None:
+            if self.max_grad_norm is None:
+                raise ValueError("HipAdamW: grad_norm is for an optimiser with max_grad_norm")
+            if grad_norm.dtype != torch.float32 or grad_norm.numel() != 1 or any(
+                    p.device != grad_norm.device for g in self.param_groups for p in g["params"] if p.grad is not None):
+                raise _lib.CinemaHipError("HipAdamW: grad_norm is one fp32 value on the parameters' device")
         entries = []
         for group in self.param_groups:
             for p in group["params"]:
@@ -81,8 +87,6 @@ class HipAdamW(torch.optim.Optimizer):
             norm = grad_norm
             if norm is None:
                 norm = _lib.binding().grad_norm([e[2].grad for e in entries], 2.0, None)
-            elif norm.dtype != torch.float32 or norm.numel() != 1 or norm.device != entries[0][1]:
-                raise _lib.CinemaHipError("HipAdamW: grad_norm is one fp32 value on the parameters' device")
             self.grad_norm = norm
         for i in range(0, len(entries), _lib.ADAMW_MAX_GROUPS):
             chunk = entries[i:i + _lib.ADAMW_MAX_GROUPS]

@@ -117,3 +117,17 @@ def test_c_entry_points_check_their_arguments():
     assert lib.cinema_adamw_step_clipped((_lib.AdamWGroup * 1)(), 1, 0, None, 1.0, None) != 0
     # struct layout of the table
     assert C.sizeof(_lib.GradTensor) == 24
+
+
+def test_clipped_step_refuses_a_norm_it_cannot_use():
+    from cinema_amd._lib import CinemaHipError
+    from cinema_amd.optim import HipAdamW
+    p = torch.nn.Parameter(torch.zeros(4))
+    p.grad = torch.ones(4)
+    with pytest.raises(ValueError, match="max_grad_norm"):
+        HipAdamW([p]).step(grad_norm=torch.ones(()))
+    opt = HipAdamW([p], max_grad_norm=1.0)
+    for bad in [torch.ones((), dtype=torch.float64), torch.ones(2), torch.ones((), device="meta")]:
+        with pytest.raises(CinemaHipError, match="grad_norm"):
+            opt.step(grad_norm=bad)
+    assert not opt.state
