@@ -91,6 +91,19 @@ Rows rows_of(const Tensor &t, int64_t k) {
 // what a node keeps: the variable itself (so that a later write to it is noticed), or the copy that was made of it
 SavedVariable saved(const Tensor &variable, const Rows &r) { return SavedVariable(r.t.is_same(variable) ? variable : r.t, false); }
 
+// A saved tensor as it came back.  Hooks on saved tensors (offloading, checkpointing) give back the values, not the layout, and a
+// leaf's .data may have been exchanged: what the kernels rely on is checked here, and strides are taken from the result.
+Tensor unpacked(const SavedVariable &saved, const char *what, const char *name, at::IntArrayRef sizes, at::ScalarType type, const Tensor &grad) {
+  Tensor t = saved.unpack();
+  if (!t.defined()) return t;
+  if (t.is_neg()) t = t.resolve_neg();
+  TORCH_CHECK(t.layout() == at::kStrided && t.sizes() == sizes && t.scalar_type() == type && t.device() == grad.device(), "cinema_amd ", what,
+              ": ", name, " was saved as ", sizes, " of ", type, " on ", grad.device(), " and came back as ", t.sizes(), " of ", t.scalar_type(),
+              " on ", t.device());
+  return t;
+}
+Tensor dense(const Tensor &t) { return t.defined() ? t.contiguous() : t; }
+
 void check_rows(const char *what, const Tensor &x) {
   TORCH_CHECK_TYPE(dtype_of(x.scalar_type()) >= 0, what, ": rows are fp32, bf16 or fp16, got ", x.scalar_type());
 }
@@ -130,10 +143,10 @@ void check_capture(const char *what, std::initializer_list<const Tensor *> input
 // ---- linear_act ------------------------------------------------------------------------------------------------------------
 struct LinearActBackward : public Node {
   SavedVariable x, w, z;
-  int64_t m, k, n, ldx;
+  int64_t m, k, n;
   int act;
   std::vector<int64_t> x_shape;
-  at::ScalarType bias_type;
+  at::ScalarType bias_type, z_type;
   std::mutex mutex;
 
   variable_list apply(variable_list &&grads) override {
@@ -151,11 +164,14 @@ struct LinearActBackward : public Node {
     if (need_w) got[1] = m ? at::empty({n, k}, o) : at::zeros({n, k}, o);
     if (need_b) got[2] = m ? at::empty({n}, o.dtype(bias_type)) : at::zeros({n}, o.dtype(bias_type));
     if (m == 0) return got;
-    const Tensor xs = x.unpack(), ws = w.unpack(), zs = z.unpack();
-    const int dt = dtype_of(g.scalar_type());
-    const void *xp = need_w ? data(xs) : nullptr, *wp = need_x ? data(ws) : nullptr;
-    const Tensor work = workspace(api.linear_work_bytes(xp, ldx, wp, m, k, n, act, dt, 1), "cinema_linear_work_bytes", g);
-    check(api.linear_backward(data(g), data(zs), zs.defined() && zs.scalar_type() == at::kFloat, xp, ldx, wp, m, k, n, act, dt,
+    const auto t = g.scalar_type();
+    const Tensor xs = unpacked(x, "linear_act", "x", x_shape, t, g), ws = dense(unpacked(w, "linear_act", "weight", {n, k}, t, g)),
+                 zs = dense(unpacked(z, "linear_act", "the pre-activation", {m, n}, z_type, g));
+    const int dt = dtype_of(t);
+    const Rows xr = need_w ? rows_of(xs, k) : Rows{Tensor(), k};
+    const void *xp = data(xr.t), *wp = need_x ? data(ws) : nullptr;
+    const Tensor work = workspace(api.linear_work_bytes(xp, xr.ld, wp, m, k, n, act, dt, 1), "cinema_linear_work_bytes", g);
+    check(api.linear_backward(data(g), data(zs), zs.defined() && z_type == at::kFloat, xp, xr.ld, wp, m, k, n, act, dt,
                               bias_type == at::kFloat, out(got[0]), out(got[1]), out(got[2]), out(work), stream_of(g)),
           "cinema_linear_backward");
     return got;
@@ -232,10 +248,10 @@ Tensor linear_act(Tensor x, Tensor w, const MaybeTensor &bias, const MaybeTensor
     node->m = m;
     node->k = k;
     node->n = n;
-    node->ldx = xr.ld;
     node->act = act;
     node->x_shape = x.sizes().vec();
     node->bias_type = b.defined() ? b.scalar_type() : x.scalar_type();
+    node->z_type = z.defined() ? z.scalar_type() : at::kFloat;
     torch::autograd::set_history(y, node);
   }
   return y;
@@ -244,7 +260,7 @@ Tensor linear_act(Tensor x, Tensor w, const MaybeTensor &bias, const MaybeTensor
 // ---- layer_norm ------------------------------------------------------------------------------------------------------------
 struct LayerNormBackward : public Node {
   SavedVariable x, w, stats;
-  int64_t m, d, ldx;
+  int64_t m, d;
   std::vector<int64_t> x_shape;
   at::ScalarType w_type;
   std::mutex mutex;
@@ -262,12 +278,14 @@ struct LayerNormBackward : public Node {
     if (need_w) got[1] = m ? at::empty({d}, o.dtype(w_type)) : at::zeros({d}, o.dtype(w_type));
     if (need_b) got[2] = m ? at::empty({d}, o.dtype(w_type)) : at::zeros({d}, o.dtype(w_type));
     if (m == 0 || !(need_x || need_w || need_b)) return got;
-    const Tensor xs = x.unpack(), ws = w.unpack(), st = stats.unpack();
+    const Rows xr = rows_of(unpacked(x, "layer_norm", "x", x_shape, g.scalar_type(), g), d);
+    const Tensor ws = dense(unpacked(w, "layer_norm", "weight", {d}, w_type, g)),
+                 st = dense(unpacked(stats, "layer_norm", "the statistics", {2, m}, at::kFloat, g));
     const int dt = dtype_of(g.scalar_type());
     Tensor work;
     if (need_w || need_b) work = workspace(api.layer_norm_work_bytes(m, d, dt), "cinema_layer_norm_work_bytes", g);
     const float *mean = st.const_data_ptr<float>();
-    check(api.layer_norm_backward(data(g), data(xs), ldx, data(ws), w_type == at::kFloat, mean, mean + m, m, d, dt, out(got[0]), out(got[1]),
+    check(api.layer_norm_backward(data(g), data(xr.t), xr.ld, data(ws), w_type == at::kFloat, mean, mean + m, m, d, dt, out(got[0]), out(got[1]),
                                   out(got[2]), out(work), stream_of(g)),
           "cinema_layer_norm_backward");
     return got;
@@ -329,7 +347,6 @@ Tensor layer_norm(Tensor x, const MaybeTensor &weight, const MaybeTensor &bias, 
     node->stats = SavedVariable(stats, false);
     node->m = m;
     node->d = d;
-    node->ldx = xr.ld;
     node->x_shape = x.sizes().vec();
     node->w_type = w_type;
     torch::autograd::set_history(y, node);

@@ -1,0 +1,97 @@
+"""linear_act and layer_norm where what they saved comes back in another layout: saved-tensor hooks, checkpointing, an exchanged
+leaf.  Equal values give equal bits, whatever their strides."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def swapped(t):
+    """the same values, the last two dimensions in the other memory order"""
+    return t.transpose(-1, -2).contiguous().transpose(-1, -2) if t.dim() > 1 else t.clone()
+
+
+def spaced(t):
+    """the same values, every row and value apart from the next, NaN in between"""
+    wide = torch.full([2 * s + 3 for s in t.shape], float("nan"), dtype=t.dtype, device=t.device)
+    v = wide[tuple(slice(1, 1 + 2 * s, 2) for s in t.shape)]
+    v.copy_(t)
+    return v
+
+
+HOOKS = {"offloaded": lambda: torch.autograd.graph.save_on_cpu(),
+         "swapped": lambda: torch.autograd.graph.saved_tensors_hooks(lambda t: t, swapped),
+         "spaced": lambda: torch.autograd.graph.saved_tensors_hooks(lambda t: t, spaced)}
+
+
+def operands(op, m, k, n, dtype, view):
+    g = torch.Generator(device="cuda").manual_seed(m + k + n)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").to(dtype)
+    wide = r(m + 2, k + 24)
+    x = wide[1:1 + m, 8:8 + k] if view == "rows_of_wider" else wide[1:1 + m, :k].contiguous()
+    if op == "linear_act":
+        return [x, r(n, k), r(n)], r(m, n)
+    return [x, r(k), r(k)], r(m, k)
+
+
+def gradients(op, leaves, dy):
+    from cinema_amd.models.mlp import layer_norm, linear_act
+    leaves = [t.detach().requires_grad_(True) for t in leaves]
+    y = linear_act(*leaves, activation="silu") if op == "linear_act" else layer_norm(*leaves)
+    return y, leaves, lambda: torch.autograd.grad(y, leaves, dy)
+
+
+@pytest.mark.parametrize("hooks", HOOKS)
+@pytest.mark.parametrize("view", ["rows_of_wider", "dense"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("op,m,k,n", [("linear_act", 40, 64, 48), ("linear_act", 1, 64, 48), ("linear_act", 1500, 72, 520), ("linear_act", 700, 33, 5),
+                                      ("layer_norm", 40, 64, 0), ("layer_norm", 33, 3000, 0), ("layer_norm", 3, 40000, 0)])
+def test_gradients_do_not_depend_on_the_saved_layout(op, m, k, n, dtype, view, hooks):
+    leaves, dy = operands(op, m, k, n, dtype, view)
+    _, _, want = gradients(op, leaves, dy)
+    with HOOKS[hooks]():
+        _, _, got = gradients(op, leaves, dy)
+    assert all(torch.equal(a, b) for a, b in zip(got(), want()))
+
+
+@pytest.mark.parametrize("op", ["linear_act", "layer_norm"])
+def test_a_leaf_whose_data_is_exchanged_for_another_layout(op):
+    leaves, dy = operands(op, 300, 64, 48, torch.float32, "rows_of_wider")
+    want = gradients(op, leaves, dy)[2]()
+    _, own, got = gradients(op, leaves, dy)
+    for t in own:
+        t.data = swapped(t.data)
+    assert all(torch.equal(a, b) for a, b in zip(got(), want))
+
+
+@pytest.mark.parametrize("op", ["linear_act", "layer_norm"])
+@pytest.mark.parametrize("bad", ["shorter", "type", "device"])
+def test_saved_values_of_another_kind_are_refused(op, bad):
+    def unpack(t):
+        return {"shorter": lambda: t[:-1], "type": lambda: t.double(), "device": lambda: t.cpu()}[bad]()
+    leaves, dy = operands(op, 40, 64, 48, torch.float32, "dense")
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        _, _, got = gradients(op, leaves, dy)
+    with pytest.raises(RuntimeError, match="came back"):
+        got()
+
+
+@pytest.mark.parametrize("early", [False, True])
+def test_checkpointed_block(early):
+    from torch.utils.checkpoint import checkpoint, set_checkpoint_early_stop
+    from cinema_amd.models.mlp import layer_norm, linear_act
+    g = torch.Generator(device="cuda").manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16()
+    wide, w, b, nw, dy = r(300, 100), r(64, 64), r(64), r(64), r(300, 64)
+
+    def block(x, *p):
+        return linear_act(layer_norm(x, p[2]), p[0], p[1], x, "gelu")
+    got = []
+    for again in (False, True):
+        leaves = [wide[:, 8:72].detach().requires_grad_(True)] + [t.clone().requires_grad_(True) for t in (w, b, nw)]
+        with set_checkpoint_early_stop(early):
+            y = checkpoint(block, *leaves, use_reentrant=False) if again else block(*leaves)
+            got.append([y.detach()] + list(torch.autograd.grad(y, leaves, dy)))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
