@@ -6,9 +6,11 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <ATen/autocast_mode.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <dlfcn.h>
@@ -119,6 +121,15 @@ void check_plain(const char *what, Tensor &t) {
   if (t.is_neg()) t = t.resolve_neg();
   TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "cinema_amd ", what, ": no forward-mode derivative");
 }
+// A tracer records the allocation of the result and not the launch that fills it: the recorded program would return whatever the
+// memory holds.  (torch.compile does not look into these calls; it breaks its graph around them and runs them as they are.)
+void check_not_traced(const char *what) {
+  using c10::impl::TorchDispatchModeTLS;
+  using c10::impl::TorchDispatchModeKey;
+  const bool traced = torch::jit::tracer::isTracing() || TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY) ||
+                      TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE) || TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FUNCTIONAL);
+  TORCH_CHECK_NOT_IMPLEMENTED(!traced, "cinema_amd ", what, ": cannot be traced (torch.jit.trace, make_fx, fake tensors)");
+}
 void check_gpu(const char *what, const Tensor &x) {
   TORCH_CHECK(x.is_cuda(), "cinema_amd ", what, " runs HIP kernels: the input must live on the GPU");
 }
@@ -189,6 +200,7 @@ const char *const ACTIVATIONS[] = {"none", "relu", "gelu", "gelu_tanh", "silu"};
 
 Tensor linear_act(Tensor x, Tensor w, const MaybeTensor &bias, const MaybeTensor &residual, const std::string &activation) {
   const char *what = "linear_act";
+  check_not_traced(what);
   int act = -1;
   for (int i = 0; i < 5; ++i)
     if (activation == ACTIVATIONS[i]) act = i;
@@ -301,6 +313,7 @@ struct LayerNormBackward : public Node {
 
 Tensor layer_norm(Tensor x, const MaybeTensor &weight, const MaybeTensor &bias, double eps) {
   const char *what = "layer_norm";
+  check_not_traced(what);
   Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
   if (x.is_cuda() && at::autocast::is_autocast_enabled(at::kCUDA)) {
     x = x.to(at::kFloat);
@@ -357,6 +370,7 @@ Tensor layer_norm(Tensor x, const MaybeTensor &weight, const MaybeTensor &bias, 
 // ---- gradient norm ---------------------------------------------------------------------------------------------------------
 // the norm of all gradients before clipping; max_norm given: clips them in place
 Tensor grad_norm(const std::vector<Tensor> &grads, double norm_type, std::optional<double> max_norm) {
+  check_not_traced("gradient norm");
   const double inf = std::numeric_limits<double>::infinity();
   TORCH_CHECK_VALUE(norm_type == 1. || norm_type == 2. || norm_type == inf, "norm_type is 1, 2 or inf, got ", norm_type);
   TORCH_CHECK_VALUE(!max_norm || *max_norm >= 0, "max_norm = ", max_norm.value_or(0));

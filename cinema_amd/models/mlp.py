@@ -18,14 +18,15 @@ def linear_act(x, weight, bias=None, residual=None, activation: str = "none"):
     strided; anything else is made contiguous first.  Under torch.autocast x, weight and residual are cast to its type, an
     fp32 bias stays.  First-order gradients for all four; with a gradient wanted, x, W and the pre-activations (2 bytes each
     for 16-bit rows, 4 for fp32 and where they are few; none without an activation) are kept.  A call that is captured into a
-    HIP graph with a gradient wanted is refused while an eager graph of the default stream still uses the same leaves."""
+    HIP graph with a gradient wanted is refused while an eager graph of the default stream still uses the same leaves; so is a
+    call under torch.jit.trace or make_fx, whose program would not have the launch."""
     return _lib.binding().linear_act(x, weight, bias, residual, activation)
 
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
     """(x - mean) / sqrt(variance + eps) * w + b over the last dimension.  weight and bias (D,) share a type, x's or fp32; each
     may be None.  The result has x's type; under torch.autocast the rows are taken as fp32, as torch does.  First-order
-    gradients; with a gradient wanted, x and two fp32 values per row are kept.  Captures as for linear_act."""
+    gradients; with a gradient wanted, x and two fp32 values per row are kept.  Captures and tracing as for linear_act."""
     return _lib.binding().layer_norm(x, weight, bias, eps)
 
 

@@ -95,3 +95,16 @@ def test_checkpointed_block(early):
             y = checkpoint(block, *leaves, use_reentrant=False) if again else block(*leaves)
             got.append([y.detach()] + list(torch.autograd.grad(y, leaves, dy)))
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_compiled_and_traced_callers():
+    """torch.compile breaks its graph around the calls and runs them; a tracer, whose program would lack the launch, is refused"""
+    from cinema_amd.models.mlp import layer_norm, linear_act
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x, w = torch.randn(40, 64, generator=g, device="cuda"), torch.randn(64, 64, generator=g, device="cuda")
+
+    def call(x):
+        return linear_act(layer_norm(x), w, activation="silu") + 1
+    assert torch.equal(torch.compile(call, backend="eager")(x), call(x))
+    with pytest.raises(NotImplementedError, match="traced"):
+        torch.jit.trace(call, x, check_trace=False)
