@@ -421,7 +421,7 @@ Tensor grad_norm(const std::vector<Tensor> &grads, double norm_type, std::option
   check(api.grad_clip(table.data(), n, kind, (float)*max_norm, out(work), norm.mutable_data_ptr<float>(), st), "cinema_grad_clip");
   for (size_t i = 0; i < grads.size(); ++i) {
     if (copies[i].defined()) const_cast<Tensor &>(grads[i]).copy_(copies[i]);
-    else if (!grads[i].is_inference()) grads[i].unsafeGetTensorImpl()->bump_version();     // written behind autograd's back
+    if (!grads[i].is_inference()) grads[i].unsafeGetTensorImpl()->bump_version();     // written behind autograd's back, copy_ below it too
   }
   return norm;
 }

@@ -1,0 +1,34 @@
+"""clip_grad_norm_, grad_norm and HipAdamW(max_grad_norm=) beside what else a program does with its gradients."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def params(*grads):
+    out = []
+    for g in grads:
+        p = torch.nn.Parameter(torch.zeros(g.shape, device=g.device, dtype=g.dtype))
+        p.grad = g
+        out.append(p)
+    return out
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_clipping_counts_as_a_write(dtype):
+    """a graph that saved a gradient notices that it was clipped since, strided gradients as well as contiguous ones"""
+    from cinema_amd.optim import clip_grad_norm_
+    base = torch.randn(50, 12, device="cuda").to(dtype)
+    for g in (base[:, :6].t(), torch.randn(30, device="cuda").to(dtype)):
+        (p,) = params(g)
+        before = p.grad._version
+        s = torch.ones((), device="cuda", dtype=dtype, requires_grad=True)
+        y = s * p.grad                          # saves the gradient
+        clip_grad_norm_([p], 0.1)
+        assert p.grad._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    with torch.inference_mode():
+        (p,) = params(torch.ones(6, 4, device="cuda", dtype=dtype).t())
+        assert abs(float(clip_grad_norm_([p], 1e-3)) - 24 ** 0.5) < 1e-5
+        assert float(p.grad.double().norm()) < 1.1e-3
