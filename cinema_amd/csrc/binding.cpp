@@ -368,6 +368,57 @@ Tensor layer_norm(Tensor x, const MaybeTensor &weight, const MaybeTensor &bias, 
 }
 
 // ---- gradient norm ---------------------------------------------------------------------------------------------------------
+typedef std::pair<uintptr_t, uintptr_t> Span;     // bytes [first, second)
+
+Span extent(const Tensor &t) {
+  int64_t last = 0;
+  for (int64_t k = 0; k < t.dim(); ++k) last += (t.size(k) - 1) * t.stride(k);
+  const uintptr_t p = (uintptr_t)t.const_data_ptr();
+  return {p, p + (last + 1) * t.element_size()};
+}
+
+// the memory of `t` as runs of neighbouring values
+void append_runs(const Tensor &t, std::vector<Span> &runs) {
+  std::vector<std::pair<int64_t, int64_t>> dims;      // stride, size
+  for (int64_t k = 0; k < t.dim(); ++k)
+    if (t.size(k) > 1) dims.emplace_back(t.stride(k), t.size(k));
+  std::sort(dims.begin(), dims.end());
+  int64_t run = 1;
+  size_t d = 0;
+  for (; d < dims.size() && dims[d].first == run; ++d) run *= dims[d].second;
+  const int64_t count = t.numel() / run;
+  TORCH_CHECK_VALUE((int64_t)runs.size() + count <= 1 << 24, "clip_grad_norm_: gradients are interleaved too finely to tell whether they overlap");
+  const uintptr_t p = (uintptr_t)t.const_data_ptr(), es = t.element_size();
+  for (int64_t n = 0; n < count; ++n) {
+    int64_t at = 0, left = n;
+    for (size_t k = d; k < dims.size(); ++k) {
+      at += left % dims[k].second * dims[k].first;
+      left /= dims[k].second;
+    }
+    runs.emplace_back(p + at * es, p + (at + run) * es);
+  }
+}
+
+// Gradients are scaled side by side, so none may share memory with another.  Where the extents of two meet (columns of one
+// table, say), their runs are compared.
+void check_apart(const std::vector<Tensor> &grads) {
+  std::vector<std::pair<Span, size_t>> all;
+  for (size_t i = 0; i < grads.size(); ++i)
+    if (grads[i].numel() > 0) all.emplace_back(extent(grads[i]), i);
+  std::sort(all.begin(), all.end());
+  std::vector<bool> meets(all.size(), false);
+  for (size_t i = 1, far = 0; i < all.size(); ++i) {      // far: the one before i that reaches furthest
+    if (all[i].first.first < all[far].first.second) meets[i] = meets[far] = true;
+    if (all[i].first.second > all[far].first.second) far = i;
+  }
+  std::vector<Span> runs;
+  for (size_t i = 0; i < all.size(); ++i)
+    if (meets[i]) append_runs(grads[all[i].second], runs);
+  std::sort(runs.begin(), runs.end());
+  for (size_t i = 1; i < runs.size(); ++i)
+    TORCH_CHECK_VALUE(runs[i].first >= runs[i - 1].second, "clip_grad_norm_: a gradient is listed twice or overlaps another");
+}
+
 // the norm of all gradients before clipping; max_norm given: clips them in place
 Tensor grad_norm(const std::vector<Tensor> &grads, double norm_type, std::optional<double> max_norm) {
   check_not_traced("gradient norm");
@@ -378,7 +429,6 @@ Tensor grad_norm(const std::vector<Tensor> &grads, double norm_type, std::option
   if (grads.empty()) return at::zeros({}, at::kFloat);
   std::vector<cinema_grad_tensor> table(grads.size());
   std::vector<Tensor> copies(grads.size());
-  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
   for (size_t i = 0; i < grads.size(); ++i) {
     const Tensor &g = grads[i];
     TORCH_CHECK_TYPE(g.layout() == at::kStrided, "gradient norm: sparse gradients are not supported");
@@ -388,25 +438,15 @@ Tensor grad_norm(const std::vector<Tensor> &grads, double norm_type, std::option
     TORCH_CHECK_VALUE(g.device() == grads[0].device(),
                       "gradient norm: the gradients are on several devices; combine the norms of each (grad_norm) instead");
     if (!g.is_contiguous()) {
-      if (max_norm) {
-        for (int64_t k = 0; k < g.dim(); ++k)
-          TORCH_CHECK_VALUE(g.stride(k) != 0 || g.size(k) <= 1, "clip_grad_norm_: an expanded gradient cannot be scaled in place");
-        for (size_t j = 0; j < i; ++j)
-          TORCH_CHECK_VALUE(!copies[j].defined() || grads[j].const_data_ptr() != g.const_data_ptr() || grads[j].sizes() != g.sizes() ||
-                                grads[j].strides() != g.strides(),
-                            "clip_grad_norm_: a gradient is listed twice or overlaps another");
-      }
+      for (int64_t k = 0; max_norm && k < g.dim(); ++k)
+        TORCH_CHECK_VALUE(g.stride(k) != 0 || g.size(k) <= 1, "clip_grad_norm_: an expanded gradient cannot be scaled in place");
       at::AutoDispatchBelowADInplaceOrView below;
       copies[i] = g.contiguous();
     }
     const Tensor &c = copies[i].defined() ? copies[i] : g;
     table[i] = {const_cast<void *>(c.const_data_ptr()), c.numel(), dt, 0};
-    if (max_norm && c.numel() > 0) spans.emplace_back((uintptr_t)table[i].g, (uintptr_t)table[i].g + c.nbytes());
   }
-  // two contiguous gradients that share memory would be scaled side by side
-  std::sort(spans.begin(), spans.end());
-  for (size_t i = 1; i < spans.size(); ++i)
-    TORCH_CHECK_VALUE(spans[i].first >= spans[i - 1].second, "clip_grad_norm_: a gradient is listed twice or overlaps another");
+  if (max_norm) check_apart(grads);
   if (!grads[0].is_cuda()) raise("gradient norm runs HIP kernels: the gradients must live on the GPU");
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::DeviceGuard guard(grads[0].device());

@@ -32,3 +32,19 @@ def test_clipping_counts_as_a_write(dtype):
         (p,) = params(torch.ones(6, 4, device="cuda", dtype=dtype).t())
         assert abs(float(clip_grad_norm_([p], 1e-3)) - 24 ** 0.5) < 1e-5
         assert float(p.grad.double().norm()) < 1.1e-3
+
+
+def test_neighbours_in_one_table_are_clipped_each():
+    """columns of one table as gradients of several parameters; a table beside a transposed view of it is refused untouched"""
+    from cinema_amd.optim import clip_grad_norm_
+    base = torch.randn(50, 12, device="cuda")
+    was = base.double()
+    ps = params(base[:, :5].t(), base[:, 5:7], base[:, 7:].t())
+    norm = float(was.norm())
+    assert abs(float(clip_grad_norm_(ps, norm / 4)) - norm) <= norm * 2.0 ** -23
+    assert bool(((base.double() - was * (norm / 4 / (norm + 1e-6))).abs() <= was.abs() * 2.0 ** -22).all())
+    square = torch.randn(8, 8, device="cuda")
+    was = square.clone()
+    with pytest.raises(ValueError, match="overlaps"):
+        clip_grad_norm_(params(square, square.t()), 0.1)
+    assert torch.equal(square, was)

@@ -37,3 +37,41 @@ def test_tracing_is_refused():
             torch.jit.trace(module, x, check_trace=False)
     with pytest.raises(RuntimeError, match="must live on the GPU"):            # outside a tracer: the check after it
         linear_act(x, w)
+
+
+def test_clipping_tells_shared_memory_from_interleaved():
+    """gradients that share a value are refused, however they are strided; neighbours in one table are not (they are refused one
+    check later here, for being on the CPU)"""
+    from cinema_amd import _lib
+    from cinema_amd.optim import clip_grad_norm_, grad_norm
+    t = torch.ones(8, 12)
+    line = torch.ones(100)
+    cube = torch.ones(4, 6, 5)
+    for a, b in [(t, t.t()), (t[:, :6], t[:, 5:]), (t[:, :6].t(), t[:, 3:9].t()), (t[::2], t[2]), (t[:, 3], t[4]), (line[::2], line[4:9]),
+                 (line[:50], line[::7]), (line[::2], line[::3]), (cube[:, :3, :4], cube[:, 2:, 1:]), (t[2:4], t[:, 1:5].t()), (line[3:4], line),
+                 (t[:, 2], t[:, 2]), (t[:0], t), (t[1:1], t[1:2].t())]:
+        ps = [torch.nn.Parameter(torch.zeros(g.shape)) for g in (a, torch.ones(3), b)]
+        for p, g in zip(ps, (a, torch.ones(3), b)):
+            p.grad = g
+        shared = bool(set(addresses(a)) & set(addresses(b)))
+        for order in (ps, ps[::-1]):
+            with pytest.raises(ValueError if shared else _lib.CinemaHipError, match="overlaps" if shared else "must live on the GPU"):
+                clip_grad_norm_(order, 1.0)
+        with pytest.raises(_lib.CinemaHipError, match="must live on the GPU"):       # reading twice is no clash
+            grad_norm(ps)
+    for parts in ([t[:, :6].t(), t[:, 6:].t()], [t[::2], t[1::2]], [line[::3], line[1::3], line[2::3]], [cube[:, :3, :4], cube[:, 3:, 2:], cube[:, :3, 4]],
+                  [t[:4], t[4:, :7], t[4:, 7:]]):
+        ps = [torch.nn.Parameter(torch.zeros(g.shape)) for g in parts]
+        for p, g in zip(ps, parts):
+            p.grad = g
+        for order in (ps, ps[::-1]):
+            with pytest.raises(_lib.CinemaHipError, match="must live on the GPU"):
+                clip_grad_norm_(order, 1.0)
+
+
+def addresses(t):
+    """where the values of `t` lie, one by one"""
+    at = torch.full(t.shape, t.storage_offset())
+    for k, (size, stride) in enumerate(zip(t.shape, t.stride())):
+        at = at + (torch.arange(size) * stride).view([-1 if j == k else 1 for j in range(t.dim())])
+    return (t.untyped_storage().data_ptr() + t.element_size() * at).flatten().tolist()
