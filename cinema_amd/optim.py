@@ -63,31 +63,31 @@ class HipAdamW(torch.optim.Optimizer):
             if grad_norm.dtype != torch.float32 or grad_norm.numel() != 1 or any(
                     p.device != grad_norm.device for g in self.param_groups for p in g["params"] if p.grad is not None):
                 raise _lib.CinemaHipError("HipAdamW: grad_norm is one fp32 value on the parameters' device")
-        entries = []
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.grad is None:
-                    continue
-                if p.dtype != torch.float32 or not p.is_contiguous() or not p.grad.is_contiguous() or not p.is_cuda:
-                    raise _lib.CinemaHipError("HipAdamW needs contiguous fp32 parameters and gradients on the GPU")
-                st = self.state[p]
-                if not st:
-                    st["step"] = 0
-                    st["exp_avg"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
-                    st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
-                st["step"] += 1
-                g = _lib.AdamWGroup()
-                g.p, g.g, g.m, g.v = p.data_ptr(), p.grad.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()
-                g.n = p.numel()
-                g.lr, (g.beta1, g.beta2) = float(group["lr"]), group["betas"]
-                g.eps, g.weight_decay, g.step = float(group["eps"]), float(group["weight_decay"]), int(st["step"])
-                entries.append((g, p.device, p))
+        todo = [(group, p) for group in self.param_groups for p in group["params"] if p.grad is not None]
+        # whatever can be refused is refused before any state changes
+        for _, p in todo:
+            if p.dtype != torch.float32 or not p.is_contiguous() or not p.grad.is_contiguous() or not p.is_cuda:
+                raise _lib.CinemaHipError("HipAdamW needs contiguous fp32 parameters and gradients on the GPU")
         norm = None
-        if self.max_grad_norm is not None and entries:
+        if self.max_grad_norm is not None and todo:
             norm = grad_norm
             if norm is None:
-                norm = _lib.binding().grad_norm([e[2].grad for e in entries], 2.0, None)
+                norm = _lib.binding().grad_norm([p.grad for _, p in todo], 2.0, None)
             self.grad_norm = norm
+        entries = []
+        for group, p in todo:
+            st = self.state[p]
+            if not st:
+                st["step"] = 0
+                st["exp_avg"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+                st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+            st["step"] += 1
+            g = _lib.AdamWGroup()
+            g.p, g.g, g.m, g.v = p.data_ptr(), p.grad.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()
+            g.n = p.numel()
+            g.lr, (g.beta1, g.beta2) = float(group["lr"]), group["betas"]
+            g.eps, g.weight_decay, g.step = float(group["eps"]), float(group["weight_decay"]), int(st["step"])
+            entries.append((g, p.device, p))
         for i in range(0, len(entries), _lib.ADAMW_MAX_GROUPS):
             chunk = entries[i:i + _lib.ADAMW_MAX_GROUPS]
             arr = (_lib.AdamWGroup * len(chunk))(*[e[0] for e in chunk])

@@ -48,3 +48,27 @@ def test_neighbours_in_one_table_are_clipped_each():
     with pytest.raises(ValueError, match="overlaps"):
         clip_grad_norm_(params(square, square.t()), 0.1)
     assert torch.equal(square, was)
+
+
+@pytest.mark.parametrize("clip", [None, 0.5])
+@pytest.mark.parametrize("bad", ["strided", "other device", "type"])
+def test_a_refused_update_changes_nothing(bad, clip):
+    """a parameter that cannot be updated is found before any other's step count, moments or values change"""
+    from cinema_amd import _lib
+    from cinema_amd.optim import HipAdamW
+    other = {"strided": lambda: torch.ones(16, device="cuda")[::2], "other device": lambda: torch.ones(8),
+             "type": lambda: torch.ones(8, device="cuda", dtype=torch.bfloat16)}[bad]()
+    p, q = params(torch.ones(8, device="cuda"), other)
+    opt = HipAdamW([p, q], lr=0.1, max_grad_norm=clip)
+    for _ in range(2):
+        with pytest.raises((_lib.CinemaHipError, ValueError)):
+            opt.step()
+    assert not opt.state and opt.grad_norm is None and not p.any() and bool((p.grad == 1).all())
+    q.grad = None                               # without it: the first step, as if none had been tried
+    opt.step()
+    assert opt.state[p]["step"] == 1
+    r = torch.nn.Parameter(torch.zeros(8, device="cuda"))
+    r.grad = p.grad.clone()
+    fresh = HipAdamW([r], lr=0.1, max_grad_norm=clip)
+    fresh.step()
+    assert torch.equal(p, r)
