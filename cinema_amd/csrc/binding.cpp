@@ -15,6 +15,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <dlfcn.h>
 #include <algorithm>
+#include <array>
 #include <limits>
 #include "../../include/cinema_hip.h"
 
@@ -140,7 +141,10 @@ void first_order_only(const char *what) {
 
 // A leaf's accumulator node runs on the stream it was made on and lives as long as an eager graph that uses the leaf.  One of
 // the default stream cannot take part in a capture: the captured backward pass would end the process from the engine's thread.
-void check_capture(const char *what, std::initializer_list<const Tensor *> inputs) {
+// Asked of the caller's own tensors: a cast (autocast's) hides its leaf behind a node.
+template <typename Inputs>
+void check_capture(const char *what, const Inputs &inputs) {
+  if (!at::GradMode::is_enabled() || std::none_of(inputs.begin(), inputs.end(), [](const Tensor *t) { return wants_grad(*t); })) return;
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
   for (const Tensor *t : inputs) {
     if (!wants_grad(*t) || t->grad_fn()) continue;
@@ -149,6 +153,14 @@ void check_capture(const char *what, std::initializer_list<const Tensor *> input
     TORCH_CHECK(!stream || stream->id() != 0, "cinema_amd ", what, ": captured with gradients while an eager graph of the default stream ",
                 "uses the same leaves; release its results first, or capture under torch.no_grad()");
   }
+}
+
+// for callers that cast their leaves themselves
+void check_capture_of(const std::string &what, const std::vector<Tensor> &tensors) {
+  std::vector<const Tensor *> on_gpu;
+  for (const Tensor &t : tensors)
+    if (t.is_cuda()) on_gpu.push_back(&t);
+  check_capture(what.c_str(), on_gpu);
 }
 
 // ---- linear_act ------------------------------------------------------------------------------------------------------------
@@ -206,6 +218,7 @@ Tensor linear_act(Tensor x, Tensor w, const MaybeTensor &bias, const MaybeTensor
     if (activation == ACTIVATIONS[i]) act = i;
   TORCH_CHECK_VALUE(act >= 0, what, ": unknown activation '", activation, "', choose from none, relu, gelu, gelu_tanh, silu");
   Tensor b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
+  if (x.is_cuda()) check_capture(what, std::array{&x, &w, &b, &r});
   if (x.is_cuda() && at::autocast::is_autocast_enabled(at::kCUDA)) {
     const auto t = at::autocast::get_autocast_dtype(at::kCUDA);
     x = x.to(t);
@@ -228,7 +241,6 @@ Tensor linear_act(Tensor x, Tensor w, const MaybeTensor &bias, const MaybeTensor
                     at::IntArrayRef(y_shape));
   check_gpu(what, x);
   const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || wants_grad(b) || wants_grad(r));
-  if (grad) check_capture(what, {&x, &w, &b, &r});
   const bool inner = grad && (x.requires_grad() || w.requires_grad() || wants_grad(b));      // something besides the residual
   Tensor y, z, wc, bc;
   Rows xr, rr;
@@ -315,6 +327,7 @@ Tensor layer_norm(Tensor x, const MaybeTensor &weight, const MaybeTensor &bias, 
   const char *what = "layer_norm";
   check_not_traced(what);
   Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+  if (x.is_cuda()) check_capture(what, std::array{&x, &w, &b});
   if (x.is_cuda() && at::autocast::is_autocast_enabled(at::kCUDA)) {
     x = x.to(at::kFloat);
     if (w.defined()) w = w.to(at::kFloat);
@@ -333,7 +346,6 @@ Tensor layer_norm(Tensor x, const MaybeTensor &weight, const MaybeTensor &bias, 
   TORCH_CHECK_VALUE(eps >= 0, what, ": eps = ", eps);
   check_gpu(what, x);
   const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(w) || wants_grad(b));
-  if (grad) check_capture(what, {&x, &w, &b});
   const at::ScalarType w_type = w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : x.scalar_type();
   Tensor y, stats, wc, bc;
   Rows xr;
@@ -472,5 +484,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bind", &bind);
   m.def("linear_act", &linear_act);
   m.def("layer_norm", &layer_norm);
+  m.def("check_capture", &check_capture_of);
   m.def("grad_norm", &grad_norm);
 }

@@ -82,6 +82,7 @@ class LatentRegressor(nn.Module):
                 x = x + h if self.residual and lin.in_features == lin.out_features else h
             return linears[-1](x)
         from .mlp import layer_norm, linear_act
+        _lib.binding().check_capture("LatentRegressor", [x] + [lin.weight for lin in linears])      # before the casts hide the leaves
         dtype = torch.bfloat16 if self.precision == "bf16" else torch.float32
         x = x.to(dtype)
         with torch.autocast("cuda", enabled=False):

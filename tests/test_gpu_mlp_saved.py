@@ -108,3 +108,47 @@ def test_compiled_and_traced_callers():
     assert torch.equal(torch.compile(call, backend="eager")(x), call(x))
     with pytest.raises(NotImplementedError, match="traced"):
         torch.jit.trace(call, x, check_trace=False)
+
+
+@pytest.mark.parametrize("op", ["linear_act", "layer_norm", "LatentRegressor"])
+def test_capture_under_casts_beside_a_living_eager_graph_is_refused(op):
+    """a cast, autocast's or the model's own, does not hide a leaf of a living eager graph from the check.  Only the refused
+    forward call is captured"""
+    from cinema_amd.models.inr_decoder import LatentRegressor
+    from cinema_amd.models.mlp import layer_norm, linear_act
+    g = torch.Generator(device="cuda").manual_seed(5)
+    r = lambda *s, t=torch.float32: torch.randn(*s, generator=g, device="cuda").to(t)
+    x = r(40, 64)
+    if op == "linear_act":
+        cases = [(x, r(64, 64).requires_grad_(True)), (x.clone().requires_grad_(True), r(64, 64))]
+        call = linear_act
+    elif op == "layer_norm":
+        cases = [(x, r(64, t=torch.bfloat16).requires_grad_(True)), (x.bfloat16().requires_grad_(True), r(64))]
+        call = layer_norm
+    else:
+        model = LatentRegressor([64], precision="bf16").cuda().requires_grad_(False)
+        cases = [(x.clone().requires_grad_(True), None)]
+        call = lambda x, _: model(x)
+    for operands in cases:
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            eager = call(*operands)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="eager graph"):
+            with torch.autocast("cuda", dtype=torch.bfloat16), torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call(*operands)
+        graph = torch.cuda.CUDAGraph()
+        with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16), torch.cuda.graph(graph):
+            y = call(*operands)
+        for _ in range(2):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, eager)
+        del eager
+    if op == "LatentRegressor":                  # the weights alone, the biases frozen
+        for lin in list(model.sequence)[::2]:
+            lin.weight.requires_grad_(True)
+        eager = call(x, None)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="eager graph"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call(x, None)
