@@ -131,11 +131,11 @@ def union_grad_norm(table_norm: torch.Tensor, shared_norm: Optional[torch.Tensor
     """2-norm of the union batch's gradient from a rank's two parts: `table_norm` over the tables that live on this rank,
     `shared_norm` over the replicated parameters after their all-reduce (None: frozen).  A rank normalises its loss by the
     union batch / number of ranks (share_batch_normaliser_), so its table gradients are that many times the union's.  One
-    all-reduce of 4 bytes; equal on every rank."""
+    all-reduce of 8 bytes; equal on every rank.  0-d, 64 bits: the square of a norm above 1.8e19 has no place in fp32."""
     _, world = world_info(process_group)
-    square = allreduce_sum((table_norm.reshape(1) / world) ** 2, process_group)
+    square = allreduce_sum((table_norm.reshape(1).double() / world) ** 2, process_group)
     if shared_norm is not None:
-        square = square + shared_norm.reshape(1) ** 2
+        square = square + shared_norm.reshape(1).double() ** 2
     return square.sqrt().reshape(())
 
 

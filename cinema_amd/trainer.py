@@ -427,7 +427,7 @@ class HotPathTrainer:
                 w.wait()
         if clipped:
             of = lambda opt: grad_norm([p for g in opt.param_groups for p in g["params"]])
-            norm = par.union_grad_norm(of(self.opt_local), None if self.opt_mlp is None else of(self.opt_mlp), self.pg)
+            norm = par.union_grad_norm(of(self.opt_local), None if self.opt_mlp is None else of(self.opt_mlp), self.pg).float()
             self.opt_local.step(grad_norm=norm)
         if self.opt_mlp is not None:
             self.opt_mlp.step(grad_norm=norm)
