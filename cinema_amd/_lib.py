@@ -195,8 +195,10 @@ SIGNATURES["cinema_layer_norm_forward"] = [_P, _I64, _P, _P, _I32, _I64, _I64, _
 SIGNATURES["cinema_layer_norm_backward"] = [_P, _P, _I64, _P, _I32, _P, _P, _I64, _I64, _I32, _P, _P, _P, _P, _P]
 SIGNATURES["cinema_grad_norm_work_bytes"] = [_I64]
 SIGNATURES["cinema_grad_norm"] = [_P, _I32, _I32, _P, _P, _P]
+SIGNATURES["cinema_grad_norm_f64"] = [_P, _I32, _I32, _P, _P, _P, _P]
 SIGNATURES["cinema_grad_clip"] = [_P, _I32, _I32, _F, _P, _P, _P]
 SIGNATURES["cinema_adamw_step_clipped"] = [C.POINTER(AdamWGroup), _I32, _I32, _P, _F, _P]
+SIGNATURES["cinema_adamw_step_clipped_f64"] = [C.POINTER(AdamWGroup), _I32, _I32, _P, _F, _P]
 _RESTYPES["cinema_layer_norm_work_bytes"] = _RESTYPES["cinema_grad_norm_work_bytes"] = C.c_int64
 
 

@@ -37,6 +37,7 @@ struct Api {
   decltype(&cinema_layer_norm_backward) layer_norm_backward;
   decltype(&cinema_grad_norm_work_bytes) grad_norm_work_bytes;
   decltype(&cinema_grad_norm) grad_norm;
+  decltype(&cinema_grad_norm_f64) grad_norm_f64;
   decltype(&cinema_grad_clip) grad_clip;
 } api = {};
 PyObject *error_class = nullptr;      // cinema_amd._lib.CinemaHipError
@@ -58,6 +59,7 @@ void bind(const std::string &path, py::object error) {
   get(api.layer_norm_backward, "cinema_layer_norm_backward");
   get(api.grad_norm_work_bytes, "cinema_grad_norm_work_bytes");
   get(api.grad_norm, "cinema_grad_norm");
+  get(api.grad_norm_f64, "cinema_grad_norm_f64");
   get(api.grad_clip, "cinema_grad_clip");
   Py_XDECREF(error_class);
   error_class = error.release().ptr();
@@ -431,8 +433,8 @@ void check_apart(const std::vector<Tensor> &grads) {
     TORCH_CHECK_VALUE(runs[i].first >= runs[i - 1].second, "clip_grad_norm_: a gradient is listed twice or overlaps another");
 }
 
-// the norm of all gradients before clipping; max_norm given: clips them in place
-Tensor grad_norm(const std::vector<Tensor> &grads, double norm_type, std::optional<double> max_norm) {
+// the norm of all gradients before clipping; max_norm given: clips them in place.  `wide`: gets the norm in 64 bits too
+Tensor take_norm(const std::vector<Tensor> &grads, double norm_type, std::optional<double> max_norm, Tensor *wide) {
   check_not_traced("gradient norm");
   const double inf = std::numeric_limits<double>::infinity();
   TORCH_CHECK_VALUE(norm_type == 1. || norm_type == 2. || norm_type == inf, "norm_type is 1, 2 or inf, got ", norm_type);
@@ -466,6 +468,12 @@ Tensor grad_norm(const std::vector<Tensor> &grads, double norm_type, std::option
   const int n = (int)grads.size();
   const Tensor work = workspace(api.grad_norm_work_bytes(n), "cinema_grad_norm_work_bytes", norm);
   void *st = stream_of(norm);
+  if (wide != nullptr) {
+    *wide = at::empty({}, norm.options().dtype(at::kDouble));
+    check(api.grad_norm_f64(table.data(), n, kind, out(work), norm.mutable_data_ptr<float>(), wide->mutable_data_ptr<double>(), st),
+          "cinema_grad_norm_f64");
+    return norm;
+  }
   if (!max_norm) {
     check(api.grad_norm(table.data(), n, kind, out(work), norm.mutable_data_ptr<float>(), st), "cinema_grad_norm");
     return norm;
@@ -477,6 +485,15 @@ Tensor grad_norm(const std::vector<Tensor> &grads, double norm_type, std::option
   }
   return norm;
 }
+Tensor grad_norm(const std::vector<Tensor> &grads, double norm_type, std::optional<double> max_norm) {
+  return take_norm(grads, norm_type, max_norm, nullptr);
+}
+// the norm as fp32, and in 64 bits
+std::pair<Tensor, Tensor> grad_norm_wide(const std::vector<Tensor> &grads, double norm_type) {
+  Tensor wide;
+  const Tensor norm = take_norm(grads, norm_type, std::nullopt, &wide);
+  return {norm, wide.defined() ? wide : norm.to(at::kDouble)};
+}
 
 }  // namespace
 
@@ -486,4 +503,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layer_norm", &layer_norm);
   m.def("check_capture", &check_capture_of);
   m.def("grad_norm", &grad_norm);
+  m.def("grad_norm_wide", &grad_norm_wide);
 }

@@ -103,10 +103,12 @@ __device__ __forceinline__ double norm_of(const double *part, int n, double *red
 }
 
 template <int KIND>
-__global__ __launch_bounds__(THREADS) void k_grad_norm(const double *part, int n, float *norm) {
+__global__ __launch_bounds__(THREADS) void k_grad_norm(const double *part, int n, float *norm, double *wide) {
   __shared__ double red[4];
   const double v = norm_of<KIND>(part, n, red);
-  if (threadIdx.x == 0) norm[0] = (float)v;
+  if (threadIdx.x != 0) return;
+  norm[0] = (float)v;
+  if (wide != nullptr) wide[0] = v;
 }
 
 template <typename T>
@@ -212,10 +214,10 @@ int sums(const cinema_grad_tensor *t, int32_t n, int32_t kind, int64_t run, doub
   return 0;
 }
 
-int norm_only(const double *part, int n_part, int32_t kind, float *norm, hipStream_t st) {
-  if (kind == 2) hipLaunchKernelGGL(k_grad_norm<2>, dim3(1), dim3(THREADS), 0, st, part, n_part, norm);
-  else if (kind == 1) hipLaunchKernelGGL(k_grad_norm<1>, dim3(1), dim3(THREADS), 0, st, part, n_part, norm);
-  else hipLaunchKernelGGL(k_grad_norm<0>, dim3(1), dim3(THREADS), 0, st, part, n_part, norm);
+int norm_only(const double *part, int n_part, int32_t kind, float *norm, double *wide, hipStream_t st) {
+  if (kind == 2) hipLaunchKernelGGL(k_grad_norm<2>, dim3(1), dim3(THREADS), 0, st, part, n_part, norm, wide);
+  else if (kind == 1) hipLaunchKernelGGL(k_grad_norm<1>, dim3(1), dim3(THREADS), 0, st, part, n_part, norm, wide);
+  else hipLaunchKernelGGL(k_grad_norm<0>, dim3(1), dim3(THREADS), 0, st, part, n_part, norm, wide);
   CINEMA_CHECK_HIP(hipGetLastError());
   return 0;
 }
@@ -224,13 +226,22 @@ int norm_only(const double *part, int n_part, int32_t kind, float *norm, hipStre
 
 extern "C" int64_t cinema_grad_norm_work_bytes(int64_t n_tensors) { return n_tensors < 0 ? -1 : (MAX_RUNS + n_tensors) * 8; }
 
-extern "C" int cinema_grad_norm(const cinema_grad_tensor *tensors, int32_t n, int32_t kind, void *work, float *norm, void *stream) {
+static int grad_norm(const char *who, const cinema_grad_tensor *tensors, int32_t n, int32_t kind, void *work, float *norm, double *wide, void *stream) {
   int64_t bytes;
-  if (check_tensors("cinema_grad_norm", tensors, n, kind, &bytes) != 0) return -1;
-  CINEMA_REQUIRE(work && norm, "cinema_grad_norm: null workspace or output");
+  if (check_tensors(who, tensors, n, kind, &bytes) != 0) return -1;
+  CINEMA_REQUIRE(work && norm, "%s: null workspace or output", who);
   int n_part;
   const int rc = sums(tensors, n, kind, run_bytes_of(bytes), (double *)work, &n_part, (hipStream_t)stream);
-  return rc != 0 ? rc : norm_only((const double *)work, n_part, kind, norm, (hipStream_t)stream);
+  return rc != 0 ? rc : norm_only((const double *)work, n_part, kind, norm, wide, (hipStream_t)stream);
+}
+
+extern "C" int cinema_grad_norm(const cinema_grad_tensor *tensors, int32_t n, int32_t kind, void *work, float *norm, void *stream) {
+  return grad_norm("cinema_grad_norm", tensors, n, kind, work, norm, nullptr, stream);
+}
+
+extern "C" int cinema_grad_norm_f64(const cinema_grad_tensor *tensors, int32_t n, int32_t kind, void *work, float *norm, double *wide, void *stream) {
+  CINEMA_REQUIRE(wide, "cinema_grad_norm_f64: null output");
+  return grad_norm("cinema_grad_norm_f64", tensors, n, kind, work, norm, wide, stream);
 }
 
 extern "C" int cinema_grad_clip(const cinema_grad_tensor *tensors, int32_t n, int32_t kind, float max_norm, void *work, float *norm, void *stream) {
@@ -242,7 +253,7 @@ extern "C" int cinema_grad_clip(const cinema_grad_tensor *tensors, int32_t n, in
   int n_part;
   const int rc = sums(tensors, n, kind, run, (double *)work, &n_part, st);
   if (rc != 0) return rc;
-  if (n_part == 0) return norm_only((const double *)work, 0, kind, norm, st);
+  if (n_part == 0) return norm_only((const double *)work, 0, kind, norm, nullptr, st);
   Runs r;
   float *out = norm;
   for (int at = 0; at < n;) {

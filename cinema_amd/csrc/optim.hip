@@ -12,7 +12,8 @@ struct AdamArgs {
   cinema_adamw_group g[CINEMA_ADAMW_MAX_GROUPS];
   float bc1[CINEMA_ADAMW_MAX_GROUPS], bc2_rsqrt[CINEMA_ADAMW_MAX_GROUPS];
   int n_groups, clear_grads;
-  const float *norm;   // device: gradient norm of a clipped step, null otherwise
+  const float *norm;   // device: gradient norm of a clipped step, in one of the two types; null otherwise
+  const double *norm64;
   float max_norm;
 };
 
@@ -31,7 +32,7 @@ __global__ __launch_bounds__(256) void k_adamw(AdamArgs a) {
   const cinema_adamw_group c = a.g[blockIdx.y];
   float scale = 1.f;
   if (CLIP) {
-    const double ratio = (double)a.max_norm / ((double)a.norm[0] + 1e-6);
+    const double ratio = (double)a.max_norm / ((a.norm64 != nullptr ? a.norm64[0] : (double)a.norm[0]) + 1e-6);
     scale = ratio >= 1. ? 1.f : (float)ratio;      // NaN stays NaN
   }
   const float step_size = c.lr / a.bc1[blockIdx.y];
@@ -66,7 +67,8 @@ __global__ __launch_bounds__(256) void k_adamw(AdamArgs a) {
 
 }  // namespace
 
-static int adamw_impl(const cinema_adamw_group *groups, int32_t n_groups, int clear_grads, const float *norm, float max_norm, void *stream) {
+static int adamw_impl(const cinema_adamw_group *groups, int32_t n_groups, int clear_grads, const float *norm, const double *norm64, float max_norm,
+                      void *stream) {
   CINEMA_REQUIRE(groups != nullptr && n_groups >= 1 && n_groups <= CINEMA_ADAMW_MAX_GROUPS,
                  "cinema_adamw_step: need 1..%d groups", CINEMA_ADAMW_MAX_GROUPS);
   AdamArgs a = {};
@@ -82,25 +84,32 @@ static int adamw_impl(const cinema_adamw_group *groups, int32_t n_groups, int cl
   a.n_groups = n_groups;
   a.clear_grads = clear_grads;
   a.norm = norm;
+  a.norm64 = norm64;
   a.max_norm = max_norm;
   if (nmax == 0) return 0;
   const unsigned gx = (unsigned)std::min<long>((nmax / 4 + 255) / 256 + 1, 2048);
-  if (norm != nullptr) hipLaunchKernelGGL(k_adamw<true>, dim3(gx, n_groups), dim3(256), 0, (hipStream_t)stream, a);
+  if (norm != nullptr || norm64 != nullptr) hipLaunchKernelGGL(k_adamw<true>, dim3(gx, n_groups), dim3(256), 0, (hipStream_t)stream, a);
   else hipLaunchKernelGGL(k_adamw<false>, dim3(gx, n_groups), dim3(256), 0, (hipStream_t)stream, a);
   CINEMA_CHECK_HIP(hipGetLastError());
   return 0;
 }
 
 extern "C" int cinema_adamw_step(const cinema_adamw_group *groups, int32_t n_groups, void *stream) {
-  return adamw_impl(groups, n_groups, 0, nullptr, 0.f, stream);
+  return adamw_impl(groups, n_groups, 0, nullptr, nullptr, 0.f, stream);
 }
 
 extern "C" int cinema_adamw_step_clear(const cinema_adamw_group *groups, int32_t n_groups, void *stream) {
-  return adamw_impl(groups, n_groups, 1, nullptr, 0.f, stream);
+  return adamw_impl(groups, n_groups, 1, nullptr, nullptr, 0.f, stream);
 }
 
 extern "C" int cinema_adamw_step_clipped(const cinema_adamw_group *groups, int32_t n_groups, int32_t clear_grads, const float *norm,
                                          float max_norm, void *stream) {
   CINEMA_REQUIRE(norm != nullptr, "cinema_adamw_step_clipped: null norm");
-  return adamw_impl(groups, n_groups, clear_grads, norm, max_norm, stream);
+  return adamw_impl(groups, n_groups, clear_grads, norm, nullptr, max_norm, stream);
+}
+
+extern "C" int cinema_adamw_step_clipped_f64(const cinema_adamw_group *groups, int32_t n_groups, int32_t clear_grads, const double *norm,
+                                             float max_norm, void *stream) {
+  CINEMA_REQUIRE(norm != nullptr, "cinema_adamw_step_clipped_f64: null norm");
+  return adamw_impl(groups, n_groups, clear_grads, nullptr, norm, max_norm, stream);
 }

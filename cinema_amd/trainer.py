@@ -25,7 +25,7 @@ from . import _lib
 from . import engine as E
 from . import parallel as par
 from .models.inr_decoder import INR_Decoder
-from .optim import HipAdamW, grad_norm
+from .optim import HipAdamW
 
 
 class SubjectStore:
@@ -426,8 +426,9 @@ class HotPathTrainer:
             if w is not None:
                 w.wait()
         if clipped:
-            of = lambda opt: grad_norm([p for g in opt.param_groups for p in g["params"]])
-            norm = par.union_grad_norm(of(self.opt_local), None if self.opt_mlp is None else of(self.opt_mlp), self.pg).float()
+            of = lambda opt: _lib.binding().grad_norm_wide([p.grad for g in opt.param_groups for p in g["params"] if p.grad is not None], 2.0)[1]
+            wide = par.union_grad_norm(of(self.opt_local), None if self.opt_mlp is None else of(self.opt_mlp), self.pg)
+            norm = (wide.float(), wide)
             self.opt_local.step(grad_norm=norm)
         if self.opt_mlp is not None:
             self.opt_mlp.step(grad_norm=norm)

@@ -550,12 +550,17 @@ typedef struct cinema_grad_tensor {
 int64_t cinema_grad_norm_work_bytes(int64_t n_tensors);
 int cinema_grad_norm(const cinema_grad_tensor *tensors /* host */, int32_t n, int32_t kind, void *work, float *norm,
                      void *stream);
+/* the norm in 64 bits beside the rounded one: it is finite where fp32 ends (3.4e38) */
+int cinema_grad_norm_f64(const cinema_grad_tensor *tensors /* host */, int32_t n, int32_t kind, void *work, float *norm,
+                         double *wide, void *stream);
 int cinema_grad_clip(const cinema_grad_tensor *tensors /* host */, int32_t n, int32_t kind, float max_norm, void *work,
                      float *norm, void *stream);
 /* cinema_adamw_step / _clear on gradients multiplied by min(1, max_norm / (norm[0] + 1e-6)) on the way; norm: a device float,
  * as cinema_grad_norm leaves it.  The gradients themselves stay as they are (or are zeroed, clear_grads != 0). */
 int cinema_adamw_step_clipped(const cinema_adamw_group *groups /* host */, int32_t n_groups, int32_t clear_grads,
                               const float *norm, float max_norm, void *stream);
+int cinema_adamw_step_clipped_f64(const cinema_adamw_group *groups /* host */, int32_t n_groups, int32_t clear_grads,
+                                  const double *norm, float max_norm, void *stream);
 
 #ifdef __cplusplus
 }

@@ -72,3 +72,42 @@ def test_a_refused_update_changes_nothing(bad, clip):
     fresh = HipAdamW([r], lr=0.1, max_grad_norm=clip)
     fresh.step()
     assert torch.equal(p, r)
+
+
+@pytest.mark.parametrize("n", [1, 1000])
+def test_clipped_update_where_the_norm_leaves_fp32(n):
+    """gradients of 3e38: their norm is beyond fp32 for n = 1000, and clipping has to leave them 0.5 / sqrt(n) each, in the update as
+    in clip_grad_norm_ before it.  The factor has fp32's least step, 2^-149: half of that is its error.  The first update is
+    lr * g / (|g| + eps / sqrt(bias correction)), within 2^-20 of lr"""
+    from cinema_amd.optim import HipAdamW, clip_grad_norm_
+    got = []
+    for fused in (False, True):
+        (p,) = params(torch.full((n,), 3e38, device="cuda"))
+        opt = HipAdamW([p], lr=0.125, weight_decay=0.0, max_grad_norm=0.5 if fused else None)
+        if not fused:
+            clip_grad_norm_([p], 0.5)
+            want = 0.5 / n ** 0.5
+            assert abs(float(p.grad[0]) - want) <= want * 2.0 ** -22 + 3e38 * 2.0 ** -150
+        opt.step()
+        got.append(p.detach().clone())
+        assert torch.equal(opt.state[p]["exp_avg"] > 0.09 * want, torch.ones_like(p, dtype=torch.bool))
+    assert bool((got[1] + 0.125).abs().max() <= 0.125 * 2.0 ** -19)
+    assert float((got[1] - got[0]).abs().max()) <= 0.125 * 2.0 ** -19
+
+
+def test_a_given_norm_as_a_pair():
+    """fp32 and 64 bits: the 64-bit one clips; both have to be there, on the gradients' device"""
+    from cinema_amd import _lib
+    from cinema_amd.optim import HipAdamW
+    outs = []
+    for given in (lambda n: None, lambda n: n.float(), lambda n: (n.float(), n)):
+        (p,) = params(torch.linspace(-1, 1, 77, device="cuda"))
+        opt = HipAdamW([p], lr=0.1, max_grad_norm=0.25)
+        opt.step(grad_norm=given(p.grad.double().norm()))
+        assert opt.grad_norm.dtype == torch.float32 and opt.grad_norm.dim() == 0
+        outs.append(p.detach().clone())
+    assert all(float((o - outs[0]).abs().max()) <= 0.1 * 2.0 ** -18 for o in outs)
+    one = torch.ones((), device="cuda")
+    for bad in [(one, one), (one, one.double().cpu()), (one.double(), one.double()), (one, torch.ones(2, device="cuda").double())]:
+        with pytest.raises(_lib.CinemaHipError, match="grad_norm"):
+            opt.step(grad_norm=bad)

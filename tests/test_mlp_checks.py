@@ -1,4 +1,6 @@
 """What linear_act, layer_norm, the gradient norm and the clipped update check on the host, without a GPU."""
+import ctypes
+
 import pytest
 import torch
 
@@ -75,3 +77,16 @@ def addresses(t):
     for k, (size, stride) in enumerate(zip(t.shape, t.stride())):
         at = at + (torch.arange(size) * stride).view([-1 if j == k else 1 for j in range(t.dim())])
     return (t.untyped_storage().data_ptr() + t.element_size() * at).flatten().tolist()
+
+
+def test_64_bit_norm_entry_points_check_their_arguments():
+    from cinema_amd import _lib
+    lib = _lib.load()
+    t = (_lib.GradTensor * 1)()
+    t[0].g, t[0].n, t[0].dtype = 256, 4, 0
+    one = ctypes.c_void_p(256)
+    for at, v in [(2, 3), (3, None), (4, None), (5, None)]:
+        a = [t, 1, 2, one, one, one, None]
+        a[at] = v
+        assert lib.cinema_grad_norm_f64(*a) != 0 and b"cinema_grad_norm_f64" in lib.cinema_last_error()
+    assert lib.cinema_adamw_step_clipped_f64((_lib.AdamWGroup * 1)(), 1, 0, None, 1.0, None) != 0
