@@ -15,28 +15,30 @@ import torch
 from . import _lib
 
 
-def _gradients(parameters):
-    if isinstance(parameters, torch.Tensor):
-        parameters = [parameters]
-    return [g for g in [p.grad for p in parameters] if g is not None]
+def _norm(parameters, norm_type, max_norm):
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [g for g in [p.grad for p in parameters] if g is not None]
+    norm = _lib.binding().grad_norm(grads, norm_type, max_norm)
+    return norm if grads or not parameters else norm.new_zeros((), device=parameters[0].device)
 
 
 def grad_norm(parameters, norm_type: float = 2.0):
     """The norm of all gradients of `parameters` (tensors with .grad, or one) taken as one vector: a 0-d fp32 device tensor, no
-    synchronisation; 0 if there are none.  norm_type 1, 2 or inf; sums in 64 bits, in a fixed order."""
-    return _lib.binding().grad_norm(_gradients(parameters), norm_type, None)
+    synchronisation; 0 if there are no gradients (on the CPU without any parameters).  norm_type 1, 2 or inf; sums in 64 bits, in
+    a fixed order."""
+    return _norm(parameters, norm_type, None)
 
 
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False):
     """torch.nn.utils.clip_grad_norm_: multiplies all gradients by min(1, max_norm / (norm + 1e-6)) in place and returns the
     norm before that (0-d fp32 device tensor).  A norm of at most max_norm writes nothing.  No synchronisation unless
     error_if_nonfinite.  A gradient may not be listed twice or overlap another: they are scaled side by side."""
-    grads = _gradients(parameters)
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     if error_if_nonfinite:
-        norm = float(_lib.binding().grad_norm(grads, norm_type, None))
+        norm = float(_norm(parameters, norm_type, None))
         if not math.isfinite(norm):
             raise RuntimeError(f"the gradients' norm of order {norm_type} is non-finite ({norm}), so they cannot be clipped")
-    return _lib.binding().grad_norm(grads, norm_type, max_norm)
+    return _norm(parameters, norm_type, max_norm)
 
 
 class HipAdamW(torch.optim.Optimizer):

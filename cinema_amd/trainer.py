@@ -426,7 +426,7 @@ class HotPathTrainer:
             if w is not None:
                 w.wait()
         if clipped:
-            of = lambda opt: _lib.binding().grad_norm_wide([p.grad for g in opt.param_groups for p in g["params"] if p.grad is not None], 2.0)[1]
+            of = lambda opt: _lib.binding().grad_norm_wide([p.grad for g in opt.param_groups for p in g["params"] if p.grad is not None], 2.0)[1].to(self.device)
             wide = par.union_grad_norm(of(self.opt_local), None if self.opt_mlp is None else of(self.opt_mlp), self.pg)
             norm = (wide.float(), wide)
             self.opt_local.step(grad_norm=norm)

@@ -111,3 +111,18 @@ def test_a_given_norm_as_a_pair():
     for bad in [(one, one), (one, one.double().cpu()), (one.double(), one.double()), (one, torch.ones(2, device="cuda").double())]:
         with pytest.raises(_lib.CinemaHipError, match="grad_norm"):
             opt.step(grad_norm=bad)
+
+
+def test_no_gradients_have_the_norm_0_where_the_parameters_are():
+    from cinema_amd.optim import clip_grad_norm_, grad_norm
+    p = torch.nn.Parameter(torch.zeros(3, device="cuda"))
+    q = torch.nn.Parameter(torch.zeros(3))
+    for call in (grad_norm, lambda ps: clip_grad_norm_(ps, 1.0), lambda ps: clip_grad_norm_(ps, 1.0, error_if_nonfinite=True)):
+        for ps, device in ((p, "cuda"), ([p], "cuda"), (iter([p, q]), "cuda"), ([q], "cpu"), ([], "cpu")):
+            n = call(ps)
+            assert n.device.type == device and n.dtype == torch.float32 and n.dim() == 0 and float(n) == 0.0
+    p.grad = torch.full((3,), 2.0, device="cuda")
+    assert grad_norm([q, p], 1.0).device.type == "cuda" and float(grad_norm(iter([q, p]), 1.0)) == 6.0
+    assert float(clip_grad_norm_(iter([q, p]), 3.0, 1.0, error_if_nonfinite=True)) == 6.0 and abs(float(p.grad[0]) - 1.0) < 1e-6
+    with pytest.raises(ValueError):
+        grad_norm([q], 3.0)
