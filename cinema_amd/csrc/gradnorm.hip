@@ -248,6 +248,7 @@ extern "C" int cinema_grad_clip(const cinema_grad_tensor *tensors, int32_t n, in
   int64_t bytes;
   if (check_tensors("cinema_grad_clip", tensors, n, kind, &bytes) != 0) return -1;
   CINEMA_REQUIRE(work && norm, "cinema_grad_clip: null workspace or output");
+  CINEMA_REQUIRE(max_norm >= 0.f, "cinema_grad_clip: max_norm = %g", (double)max_norm);
   hipStream_t st = (hipStream_t)stream;
   const int64_t run = run_bytes_of(bytes);
   int n_part;

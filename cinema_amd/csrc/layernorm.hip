@@ -444,6 +444,7 @@ extern "C" int cinema_layer_norm_forward(const void *x, int64_t ldx, const void 
                                          int32_t dtype, void *y, float *mean, float *rstd, void *stream) {
   if (check_sizes("cinema_layer_norm_forward", M, D, dtype) != 0) return -1;
   CINEMA_REQUIRE(x && y && ldx >= D && (mean == nullptr) == (rstd == nullptr), "cinema_layer_norm_forward: null operand, or a row stride below the row");
+  CINEMA_REQUIRE(eps >= 0.f, "cinema_layer_norm_forward: eps = %g", (double)eps);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == CINEMA_DT_F32) return forward_t<float, float>(x, ldx, w, b, M, D, eps, y, mean, rstd, st);
   if (dtype == CINEMA_DT_BF16) return w_f32 ? forward_t<bf16_t, float>(x, ldx, w, b, M, D, eps, y, mean, rstd, st) : forward_t<bf16_t, bf16_t>(x, ldx, w, b, M, D, eps, y, mean, rstd, st);

@@ -104,12 +104,12 @@ extern "C" int cinema_adamw_step_clear(const cinema_adamw_group *groups, int32_t
 
 extern "C" int cinema_adamw_step_clipped(const cinema_adamw_group *groups, int32_t n_groups, int32_t clear_grads, const float *norm,
                                          float max_norm, void *stream) {
-  CINEMA_REQUIRE(norm != nullptr, "cinema_adamw_step_clipped: null norm");
+  CINEMA_REQUIRE(norm != nullptr && max_norm >= 0.f, "cinema_adamw_step_clipped: null norm, or max_norm = %g", (double)max_norm);
   return adamw_impl(groups, n_groups, clear_grads, norm, nullptr, max_norm, stream);
 }
 
 extern "C" int cinema_adamw_step_clipped_f64(const cinema_adamw_group *groups, int32_t n_groups, int32_t clear_grads, const double *norm,
                                              float max_norm, void *stream) {
-  CINEMA_REQUIRE(norm != nullptr, "cinema_adamw_step_clipped_f64: null norm");
+  CINEMA_REQUIRE(norm != nullptr && max_norm >= 0.f, "cinema_adamw_step_clipped_f64: null norm, or max_norm = %g", (double)max_norm);
   return adamw_impl(groups, n_groups, clear_grads, nullptr, norm, max_norm, stream);
 }

@@ -524,7 +524,7 @@ int cinema_linear_backward(const void *dy, const void *z, int32_t z_f32, const v
                            void *stream);
 
 /* Layer norm of rows of D values: y = (x - mean) rstd w + b, rstd = 1 / sqrt(variance + eps); w, b [D] may be NULL, fp32
- * (w_f32 != 0) or of the rows' type.  mean, rstd [M] fp32: what the backward pass reads (NULL if no gradient is wanted).
+ * (w_f32 != 0) or of the rows' type; eps >= 0.  mean, rstd [M] fp32: what the backward pass reads (NULL if no gradient is wanted).
  * Backward: dx [M x D], dw, db [D] (w's type); each may be NULL.  Every sum has a fixed order.
  * work: cinema_layer_norm_work_bytes bytes, NULL if neither dw nor db is wanted. */
 int64_t cinema_layer_norm_work_bytes(int64_t M, int64_t D, int32_t dtype);
@@ -538,7 +538,7 @@ int cinema_layer_norm_backward(const void *dy, const void *x, int64_t ldx, const
  * norm = (sum |g|^p)^(1/p) over all values of all tensors, kind = p = 1 or 2, kind 0: max |g|; sums in 64 bits, fixed order.
  * cinema_grad_clip then multiplies every gradient by min(1, max_norm / (norm + 1e-6)) in place; nothing is written where that
  * is 1.  A NaN norm gives NaN gradients, an infinite one zeros (NaN where the gradient is infinite).  The tensors are
- * contiguous and do not overlap.  norm: one device float, the norm before clipping.
+ * contiguous and do not overlap; max_norm >= 0.  norm: one device float, the norm before clipping.
  * work: cinema_grad_norm_work_bytes(number of tensors) bytes. */
 typedef struct cinema_grad_tensor {
   void *g;       /* device */

@@ -90,3 +90,20 @@ def test_64_bit_norm_entry_points_check_their_arguments():
         a[at] = v
         assert lib.cinema_grad_norm_f64(*a) != 0 and b"cinema_grad_norm_f64" in lib.cinema_last_error()
     assert lib.cinema_adamw_step_clipped_f64((_lib.AdamWGroup * 1)(), 1, 0, None, 1.0, None) != 0
+
+
+def test_c_entry_points_refuse_bounds_that_would_turn_gradients():
+    """a negative or undefined bound is an error before anything is launched (a negative factor would turn every gradient)"""
+    from cinema_amd import _lib
+    lib = _lib.load()
+    t = (_lib.GradTensor * 1)()
+    t[0].g, t[0].n, t[0].dtype = 256, 4, 0
+    one, group = ctypes.c_void_p(256), (_lib.AdamWGroup * 1)()
+    for bad in (-1.0, -1e-30, float("nan"), -float("inf")):
+        assert lib.cinema_grad_clip(t, 1, 2, bad, one, one, None) != 0
+        assert b"max_norm" in lib.cinema_last_error()
+        for step in (lib.cinema_adamw_step_clipped, lib.cinema_adamw_step_clipped_f64):
+            assert step(group, 1, 0, one, bad, None) != 0
+            assert b"max_norm" in lib.cinema_last_error()
+        assert lib.cinema_layer_norm_forward(one, 8, None, None, 0, 4, 8, bad, _lib.DT_F32, one, None, None, None) != 0
+        assert b"eps" in lib.cinema_last_error()
