@@ -752,11 +752,17 @@ template <typename T, bool CA, bool CB>
 int product(const GemmOperand &A, const GemmOperand &B, Epilogue e, int dt, void *part, hipStream_t st) {
   Plan p = plan_product(A.ext, B.ext, A.red, dt, e.res != nullptr || e.z != nullptr ? EPI_HEAVY : e.act != ACT_NONE ? EPI_ACT : EPI_SUMS);
   // rows that are no multiple of 16 bytes: a residual's loads and z's stores take two lines each, and 64 x 64 tiles have the
-  // waves to hide that.  8191 x 1283 outputs, bf16, gelu and residual, 128 against 64: r = 256 28 -> 22 us, 512 33 -> 30,
-  // 1024 45 -> 44; z: 27 -> 23, 32 -> 30, 43 -> 43.
-  const int64_t bytes_of_r = A.red * (int64_t)sizeof(T);
-  if (sizeof(T) == 2 && p.splits == 1 && p.tile > 64 && B.ext % 8 != 0 && up(A.ext, 64) * up(B.ext, 64) < (1 << 24) &&
-      ((e.res != nullptr && bytes_of_r <= 2048) || (e.z != nullptr && bytes_of_r <= 1024))) {
+  // waves to hide that -- while the outputs are few enough and r is short enough that the epilogue counts for more than what the
+  // smaller tiles read again.  16-bit types, gelu, residual (z is alike), us with the tiles of the plan -> with 64 x 64:
+  //   r =              200            264            512            768           1024
+  //   4000 x 1001   12.5 ->  9.2   13.1 -> 10.2   14.2 -> 11.1   17.4 -> 13.8          (2048 x 1283)  17.6 -> 12.9
+  //   12000 x 1001  27.2 -> 22.2   29.0 -> 24.7   31.5 -> 28.5   37.9 -> 36.7          (8191 x 1283)  43.0 -> 45.8
+  //   20000 x 777   28.8 -> 28.9   35.7 -> 31.7   40.8 -> 37.0   49.8 -> 48.2
+  //   12000 x 1502  34.5 -> 32.3   37.3 -> 36.0   41.8 -> 42.1   51.1 -> 55.1
+  //   20000 x 1502  48.2 -> 49.8   52.4 -> 56.2   58.8 -> 68.3   77.9 -> 89.3
+  //   50000 x 1001  80.3 -> 84.1   87.8 -> 91.6    102 -> 115     132 -> 167
+  if (sizeof(T) == 2 && p.splits == 1 && p.tile > 64 && B.ext % 8 != 0 && (e.res != nullptr || e.z != nullptr) && A.ext * B.ext <= (1 << 24) &&
+      A.red <= (A.ext * B.ext <= (1 << 22) ? 1024 : 512)) {
     p.tile = 64;
     p.deep = false;
     p.ti = up(A.ext, 64);

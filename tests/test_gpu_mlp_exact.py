@@ -168,3 +168,11 @@ def test_layer_norm_by_the_norm(m, d, dtype):
         allowed = U[got.dtype] + (64 + math.sqrt(m) + math.sqrt(d)) * 2.0 ** -22 * (64 if d < 16 else 1)
         assert allowed < 0.05
         near(got, want[name], allowed, f"{name} of {m}x{d} {dtype}")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n", [(4000, 264, 1001), (12001, 200, 777), (16384, 512, 1023), (16400, 512, 1023), (12000, 513, 1001), (30001, 72, 1003),
+                                   (4100, 1024, 1022), (4100, 1032, 1022), (4110, 1024, 1022)])
+def test_linear_sums_are_whole_where_odd_rows_change_tiles(m, k, n, dtype):
+    """either side of where a residual or a kept z on odd rows takes smaller tiles: 2^24 outputs and 512 values of r, 2^22 and 1024"""
+    check_exact(m, k, n, dtype, "relu", 1 << 14)
