@@ -740,13 +740,6 @@ int pack_operands(const void *&x, int64_t &ldx, int64_t xr, int64_t xc, const vo
   return 0;
 }
 
-// 256 x 256: one workgroup of eight waves on a compute unit; the 16-bit types only (fp32 gains nothing from it)
-template <typename T, bool CA, bool CB>
-int launch_large(const GemmOperand &A, const GemmOperand &B, const Epilogue &e, const Plan &p, hipStream_t st) {
-  if constexpr (sizeof(T) == 2) return launch_tile<T, CA, CB, 256, 256, 2, 4, 2>(A, B, e, p, st);
-  return -1;
-}
-
 // C = A B^T with the epilogue; part = workspace of plan.part_bytes
 template <typename T, bool CA, bool CB>
 int product(const GemmOperand &A, const GemmOperand &B, Epilogue e, int dt, void *part, hipStream_t st) {
@@ -774,8 +767,10 @@ int product(const GemmOperand &A, const GemmOperand &B, Epilogue e, int dt, void
   if (p.tile == 64 && p.deep) rc = launch_tile<T, CA, CB, 64, 64, 2, 2, sizeof(T) == 2 ? 4 : 2>(A, B, e, p, st);
   else if (p.tile == 64) rc = launch_tile<T, CA, CB, 64, 64, 2, 2, 2>(A, B, e, p, st);
   else if (p.tile == 128 && p.deep) rc = launch_tile<T, CA, CB, 128, 128, 2, 2, sizeof(T) == 2 ? 4 : 2>(A, B, e, p, st);
-  else if (p.tile == 128 || sizeof(T) == 4) rc = launch_tile<T, CA, CB, 128, 128, 2, 2, 2>(A, B, e, p, st);
-  else rc = launch_large<T, CA, CB>(A, B, e, p, st);
+  else if (p.tile == 128) rc = launch_tile<T, CA, CB, 128, 128, 2, 2, 2>(A, B, e, p, st);
+  // 256 x 256: one workgroup of eight waves on a compute unit; no plan of fp32 has it (it gains nothing there)
+  else if constexpr (sizeof(T) == 2) rc = launch_tile<T, CA, CB, 256, 256, 2, 4, 2>(A, B, e, p, st);
+  else CINEMA_REQUIRE(false, "linear layer: no kernel for tiles of %d", p.tile);
   if (rc != 0 || p.splits == 1) return rc;
   const int64_t groups = A.ext * (p.ldp >> 3);
   hipLaunchKernelGGL(k_linear_join<T>, dim3((unsigned)std::min<int64_t>(up(groups, 256), 4096)), dim3(256), 0, st, e, A.ext, B.ext, p.splits);

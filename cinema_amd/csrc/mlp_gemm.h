@@ -22,8 +22,6 @@ typedef _Float16 f16_t;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-__device__ __forceinline__ float to_f32(f16_t x) { return (float)x; }
-
 // memory order of one operand; ext = extent of i (or j), red = extent of r, ld = elements between rows
 struct GemmOperand { const void *p; int64_t ld; int64_t ext; int64_t red; };
 
