@@ -252,7 +252,8 @@ Tensor linear_act(Tensor x, Tensor w, const MaybeTensor &bias, const MaybeTensor
     y = at::empty(y_shape, x.options());
     // 16-bit rows keep fp16 pre-activations; where few of them make a gradient their rounding would show, and fp32 costs nothing
     if (inner && act != CINEMA_ACT_NONE)
-      z = at::empty({m, n}, x.options().dtype(x.scalar_type() == at::kFloat || m * n <= 1 << 18 || n * k <= 2048 ? at::kFloat : at::kHalf));
+      z = at::empty({m, n}, x.options().dtype(x.scalar_type() == at::kFloat || m * n <= 1 << 18 || n * k <= 2048 || m * k <= 256
+                                                               ? at::kFloat : at::kHalf));
     xr = rows_of(x, k);
     wc = w.contiguous();
     if (b.defined()) bc = b.contiguous();

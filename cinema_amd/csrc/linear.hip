@@ -808,11 +808,15 @@ bool small_backward(int64_t M, int64_t K, int64_t N, int dt) {
   return std::max(M, N) <= (f32 ? SMALL_R : SMALL_R / 2) && M * K * N <= (f32 ? 32 << 20 : 17 << 20);
 }
 
-// dz of a smooth activation is rounded to 16 bits for the matrix unit.  Where few values of it (M N) or few sums over it (N K)
-// make the gradients, those roundings do not average out (971 x 1 x 3: dW off by 0.006 of its norm, 0.0017 is its own rounding),
-// and the products are small: they then run in fp32.
+// dz of a smooth activation is rounded to 16 bits for the matrix unit, each value by at most U of itself (2^-8 or 2^-11) and by
+// 0.41 U in the root mean square.  A gradient that sums them with independent signs is then off by 0.41 U |terms| in the 2-norm,
+// |terms| = sqrt(sum of (dz w)^2), as much as its own rounding adds: 0.0024 together against 0.0017 (bf16).  That is relative to
+// the gradient if its norm is near |terms|, which it is within 1 / sqrt(2 n) for n values.  Where one of the gradients has few
+// (dx M K, dW N K) or comes from few roundings (M N), its norm may lie far below: dW of 971 x 1 x 3 was off by 0.006, dx of
+// 3 x 1 x 4000 by 0.013.  The products of such a backward pass are small, so all of them run in fp32 there; the bounds keep
+// 1 / sqrt(2 n) below 5 % for dx (whose fp32 copy of W would cost most), 2 % for dW and 1 % for dz.
 bool wide_backward(int64_t M, int64_t K, int64_t N, int act, int dt) {
-  return dt != CINEMA_DT_F32 && act != ACT_NONE && act != ACT_RELU && (N * K <= 2048 || M * N <= 8192);
+  return dt != CINEMA_DT_F32 && act != ACT_NONE && act != ACT_RELU && (N * K <= 2048 || M * N <= 8192 || M * K <= 256);
 }
 
 struct BackwardPlan { int64_t ldz, dz, db, pack, part, total; };

@@ -176,3 +176,28 @@ def test_layer_norm_by_the_norm(m, d, dtype):
 def test_linear_sums_are_whole_where_odd_rows_change_tiles(m, k, n, dtype):
     """either side of where a residual or a kept z on odd rows takes smaller tiles: 2^24 outputs and 512 values of r, 2^22 and 1024"""
     check_exact(m, k, n, dtype, "relu", 1 << 14)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("m,k,n", [(1, 1, 10000), (3, 1, 4000), (9, 2, 4096), (2, 30, 8000), (1, 200, 9000), (64, 1, 4099), (256, 1, 2100), (1, 8, 300000),
+                                   (971, 1, 3), (20000, 3, 2)])
+def test_linear_gradients_of_few_values_by_the_norm(m, k, n, act, dtype):
+    """dx of few values from many features, as dW of few from many rows: dz stays in 32 bits, so a gradient is off by its own rounding,
+    U of each value at most, and by the fp32 sums, relative to the norm of what is summed.  Ten inputs, as a single one may be lucky"""
+    from cinema_amd.models.mlp import linear_act
+    for seed in range(10):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        rn = lambda *s, c=1.0: (torch.randn(*s, generator=g, device="cuda") * c).to(dtype)
+        x, w, b, dy = rn(m, k), rn(n, k, c=1 / math.sqrt(k)), rn(n, c=0.2), rn(m, n, c=0.1)
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+        dx, dw, db = torch.autograd.grad(linear_act(*leaves, None, act), leaves, dy)
+        z = x.double() @ w.double().t() + b.double()
+        dz = dy.double() * slope64(z, act)
+        W, X, one = w.double(), x.double(), torch.ones(1, m, device="cuda", dtype=torch.float64)
+        for got, a, c in ((dx, dz, W), (dw, dz.t(), X), (db, one, dz)):
+            want = (a @ c).view_as(got)
+            # a term's own error, of the activation and of z: (|z| + 4)^2 2^-21 of it, far below 2^-16; they add like their signs
+            terms = float(((a * a) @ (c * c)).sum().sqrt())
+            allowed = U[dtype] * float(want.norm()) + terms * (2.0 ** -15 + (8 + math.sqrt(max(m, n)) + math.sqrt(k)) * 2.0 ** -22)
+            assert float((got.double() - want).norm()) <= allowed, (seed, float((got.double() - want).norm()) / float(want.norm()), allowed / float(want.norm()))
