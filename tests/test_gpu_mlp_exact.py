@@ -201,3 +201,28 @@ def test_linear_gradients_of_few_values_by_the_norm(m, k, n, act, dtype):
             terms = float(((a * a) @ (c * c)).sum().sqrt())
             allowed = U[dtype] * float(want.norm()) + terms * (2.0 ** -15 + (8 + math.sqrt(max(m, n)) + math.sqrt(k)) * 2.0 ** -22)
             assert float((got.double() - want).norm()) <= allowed, (seed, float((got.double() - want).norm()) / float(want.norm()), allowed / float(want.norm()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [8, 4000])
+def test_gelu_keeps_its_relative_accuracy_far_below_zero(rows, dtype):
+    """z Phi(z) and its slope at z from -0.02 to -12, where they fall to 1e-31: relative to the value, half a step of the type (the slope
+    leaves its root at -0.75 out), 2^-17 for the 16-bit types' polynomial, and for every type what the exponent makes of its own
+    rounding: z^2 2^-24 for the square and its factor, z^2 2^-24 more for z / sqrt 2 inside the fp32 library function, 16 * 2^-24 for
+    the products"""
+    from cinema_amd.models.mlp import linear_act
+    z = -torch.linspace(0.02, 12.0, rows, device="cuda").to(dtype)
+    x = z.view(-1, 1).clone().requires_grad_(True)
+    w = torch.ones(1, 1, device="cuda", dtype=dtype)
+    y = linear_act(x, w, None, None, "gelu")
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    zd = z.double()
+    cdf = 0.5 * torch.special.erfc(-zd / math.sqrt(2))
+    slope = cdf + zd * torch.exp(-0.5 * zd * zd) / math.sqrt(2 * math.pi)
+    smallest = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}[dtype]
+    rel = U[dtype] + (0 if dtype == torch.float32 else 2.0 ** -17) + 2 * zd * zd * 2.0 ** -24 + 16 * 2.0 ** -24
+    for got, want, keep in ((y.detach().flatten(), zd * cdf, zd < 0), (dx.flatten(), slope, (zd + 0.75).abs() > 0.2)):
+        # the slope is the difference of two terms: its error counts against their sum of magnitudes
+        size = want.abs() if want is not slope else cdf + (slope - cdf).abs()
+        bad = ((got.double() - want).abs() > rel * size + smallest)[keep]
+        assert not bad.any(), (float(zd[keep][bad][0]), float(got.double()[keep][bad][0]), float(want[keep][bad][0]))
