@@ -4,7 +4,7 @@
 // more scales; every scaling workgroup adds the partials itself, in the same order, so there is no launch between and no
 // atomic.  Sums are 64-bit: a gradient's square neither overflows nor vanishes, and the order does not show in fp32.
 // c = 1 writes nothing.  Bound by HBM: each gradient is read once, and read and written once more where c < 1.  60 tensors, 79 M
-// bf16 values: sums 24 us = 6.4 TB/s, scaling 51 us = 6.2 TB/s (the last-level cache holds part of them).
+// bf16 values: sums 28 us = 5.7 TB/s, scaling 51 us = 6.2 TB/s (the last-level cache holds part of them).
 #include "rows.h"
 #include <algorithm>
 

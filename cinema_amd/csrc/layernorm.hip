@@ -26,7 +26,7 @@ __device__ __forceinline__ float row_sum(float x, float *red, int slot) {
 // NW == 1: a workgroup of four waves, each with its own rows; else a workgroup of NW waves on one row after the other.  Weights
 // stay in registers over the rows (read per row they would be as many bytes from the L2 as the rows from memory), and the
 // next row is under way while this one is reduced.  bf16: 16384 x 4096 64 us = 4.2 TB/s (94 with weights read per row), 25000 x 512
-// 12 us = 4.3 TB/s.
+// 13 us = 3.9 TB/s.
 template <typename T, typename W, int NW, int CH>
 __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void k_norm_fwd(const T *x, int64_t ldx, const W *w, const W *b, int64_t M, int D, float eps,
                                                                       T *y, float *mean, float *rstd) {
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void k_norm_fwd(const T *x
   }
 }
 
-// any D: 1024 threads walk the row three times
+// any D: 1024 threads walk the row three times.  2048 x 16384 fp32 76 us = 3.5 TB/s, 4096 x 32768 bf16 160 us = 3.4
 template <typename T, typename W>
 __global__ __launch_bounds__(1024) void k_norm_fwd_long(const T *x, int64_t ldx, const W *w, const W *b, int64_t D, float eps, T *y, float *mean,
                                                         float *rstd) {
@@ -139,7 +139,7 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_long(const T *x, int64_t ldx,
 
 // Backward.  A workgroup walks over rows (its waves each over their own for NW == 1) and keeps the sums g h and g of its
 // columns in registers; they leave as one row of partials per workgroup, k_norm_join adds those in a fixed order.
-// PARAMS: dw / db wanted.  16384 x 4096 bf16 with fp32 weights: 97 us = 4.2 TB/s, and 6 us for the join.
+// PARAMS: dw / db wanted.  16384 x 4096 bf16 with fp32 weights: 96 us = 4.2 TB/s, and 6 us for the join.
 template <typename T, typename W, int NW, int CH, bool PARAMS>
 __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void k_norm_bwd(const T *g, const T *x, int64_t ldx, const W *w, const float *mean,
                                                                       const float *rstd, int64_t M, int D, T *dx, float *part, W *dw, W *db) {
@@ -253,7 +253,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void k_norm_bwd(const T *g
     }
 }
 
-// any D: dx by 1024 threads per row in two walks
+// any D: dx by 1024 threads per row in two walks.  2048 x 16384 fp32 116 us = 3.5 TB/s, 4096 x 32768 bf16 390 us = 2.1
 template <typename T, typename W>
 __global__ __launch_bounds__(1024) void k_norm_bwd_long(const T *g, const T *x, int64_t ldx, const W *w, const float *mean, const float *rstd,
                                                         int64_t D, T *dx) {
@@ -290,7 +290,7 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(const T *g, const T *x, 
   }
 }
 
-// any D: partial dw, db of a block of rows; a thread has one column
+// any D: partial dw, db of a block of rows; a thread has one column.  2048 x 16384 fp32 50 us, 4096 x 32768 bf16 161 us
 template <typename T>
 __global__ __launch_bounds__(256) void k_norm_params_long(const T *g, const T *x, int64_t ldx, const float *mean, const float *rstd, int64_t M,
                                                           int64_t D, int64_t rows, float *part) {

@@ -3,9 +3,9 @@
 // x [M][K], W [N][K], y [M][N] in fp32, bf16 or fp16; every sum and the whole epilogue in fp32, y, dx and dW rounded once.
 // 16-bit types keep z in fp16 (11 bits; act' of a bf16 z would add as much error as the rounding of the gradient itself, and
 // beyond 65504 act' does not change, so the range is enough) where z is large, in fp32 where it is small; fp32 keeps it as it is.
-// Large 16-bit products take dz rounded to the matrix instruction's input type, whose errors average out over the sums; where few
-// values or few sums make a gradient they do not, and dz stays in 32 bits there (small_backward and wide_backward).  db is
-// summed before the rounding.
+// Large 16-bit products take dz rounded to the matrix instruction's input type, which adds as much to a gradient as its own rounding;
+// where few values or few sums make a gradient it could add more, and dz stays in 32 bits there (small_backward and
+// wide_backward, which derives it).  db is summed before the rounding.
 #include "mlp_gemm.h"
 #include <algorithm>
 #include <cmath>
@@ -288,8 +288,10 @@ __device__ __forceinline__ void write_tile(const f32x16 (&acc)[G::TI][G::TJ], in
 }
 
 // One workgroup = one BI x BJ tile of one split.  Bound by the matrix unit and the L2 (its 32 KB or 64 KB of operands a step);
-// the 256 x 256 tile, alone on its compute unit, adds its epilogue on top.  bf16: 32768 x 1024 x 4096 235 us = 1170 TFLOP/s, 280
-// with gelu; 25000 x 512 x 512 21 us, 33 with gelu, residual and z (129 MB: 3.9 TB/s).  fp32: 16384 x 2048 x 1024 482 us = 143.
+// the 256 x 256 tile, alone on its compute unit, adds its epilogue on top.  Whole calls back to back over three sets of inputs, bf16:
+// 32768 x 1024 x 4096 269 us = 1020 TFLOP/s, 294 with bias and gelu_tanh, 330 with gelu; 25000 x 512 x 512 21 us, 28 with gelu, 33
+// with a residual too.  fp32: 16384 x 2048 x 1024 485 us = 142.  Counters of the wide one: the matrix unit is busy 48 % of the
+// cycles, 45 beside gelu_tanh; the vector unit 14 % and 27.
 template <typename T, bool CA, bool CB, int BI, int BJ, int WI, int WJ, int RING>
 __global__ __launch_bounds__(WI *WJ * 64, 2) void k_linear(GemmOperand A, GemmOperand B, Epilogue e, int tiles_i, int tiles_j, int64_t per_split) {
   typedef GemmTile<T, CA, CB, BI, BJ, WI, WJ, RING> G;
@@ -423,7 +425,7 @@ __global__ __launch_bounds__(256) void k_linear_rows(const T *x, int64_t ldx, co
 
 // dz = dy * act'(z) and the column sums of dz over the block's rows.  A workgroup takes 512 columns (64 lanes x 8) and `rows`
 // rows, its eight waves every eighth row, two of them under way; sums of the waves meet in LDS.  dz has rows of ldz values, zeros behind the N'th (the
-// products read whole chunks).  dz == null: only the sums.  Bound by memory: 25000 x 512 bf16, 77 MB, 18 us = 4.2 TB/s.
+// products read whole chunks).  dz == null: only the sums.  Bound by memory: 25000 x 512 bf16, 77 MB, 21 us = 3.7 TB/s.
 template <typename T, typename TO, bool Z32>
 __global__ __launch_bounds__(512) void k_linear_dz(const T *dy, const void *zv, TO *dz, int64_t ldz, float *part, int64_t M, int64_t N, int64_t rows,
                                                    int act, void *db, int db_f32) {
@@ -608,7 +610,7 @@ __global__ __launch_bounds__(256) void k_linear_pack(Pack a, Pack b) {
 }
 
 // out[col] = sum over P partial rows, in a fixed order: 32 columns per workgroup, 32 groups of lanes over the partials
-// (511 rows of 512: 4.6 us; 64 columns and four waves per workgroup took 60)
+// (511 rows of 512: 4.8 us; 64 columns and four waves per workgroup took 60)
 template <typename T>
 __global__ __launch_bounds__(1024) void k_column_join(const float *part, int P, int64_t N, void *out, int out_f32) {
   __shared__ float red[32][33];
