@@ -57,21 +57,15 @@ class HipAdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None, grad_norm=None):
-        """grad_norm: with max_grad_norm, the norm to clip by (0-d fp32 device tensor) in place of this optimiser's own
-        gradients' -- for a step whose gradients are spread over several optimisers or processes.  It may also be a pair of
-        that and the same norm as a 0-d fp64 tensor, which is then what clips: fp32 ends at 3.4e38, and an infinite norm makes
-        every gradient zero."""
-        wide = None
-        if isinstance(grad_norm, tuple):
-            grad_norm, wide = grad_norm
-            if wide.dtype != torch.float64 or wide.numel() != 1 or wide.device != grad_norm.device:
-                raise _lib.CinemaHipError("HipAdamW: the second grad_norm is the first one's value in fp64, on the same device")
+        """grad_norm: with max_grad_norm, the norm to clip by (0-d fp32 or fp64 device tensor) in place of this optimiser's own
+        gradients' -- for a step whose gradients are spread over several optimisers or processes.  fp32 ends at 3.4e38, and an
+        infinite norm makes every gradient zero."""
         if grad_norm is not None:
             if self.max_grad_norm is None:
                 raise ValueError("HipAdamW: grad_norm is for an optimiser with max_grad_norm")
-            if grad_norm.dtype != torch.float32 or grad_norm.numel() != 1 or any(
+            if grad_norm.dtype not in (torch.float32, torch.float64) or grad_norm.numel() != 1 or not grad_norm.is_cuda or any(
                     p.device != grad_norm.device for g in self.param_groups for p in g["params"] if p.grad is not None):
-                raise _lib.CinemaHipError("HipAdamW: grad_norm is one fp32 value on the parameters' device")
+                raise _lib.CinemaHipError("HipAdamW: grad_norm is one fp32 or fp64 value on the parameters' device, a GPU")
         todo = [(group, p) for group in self.param_groups for p in group["params"] if p.grad is not None]
         # whatever can be refused is refused before any state changes
         for _, p in todo:
@@ -79,10 +73,7 @@ class HipAdamW(torch.optim.Optimizer):
                 raise _lib.CinemaHipError("HipAdamW needs contiguous fp32 parameters and gradients on the GPU")
         norm = None
         if self.max_grad_norm is not None and todo:
-            norm = grad_norm
-            if norm is None:
-                norm, wide = _lib.binding().grad_norm_wide([p.grad for _, p in todo], 2.0)
-            self.grad_norm = norm
+            self.grad_norm, norm = _lib.binding().grad_norm_wide([p.grad for _, p in todo], 2.0) if grad_norm is None else (grad_norm.float(), grad_norm)
         entries = []
         for group, p in todo:
             st = self.state[p]
@@ -102,8 +93,8 @@ class HipAdamW(torch.optim.Optimizer):
             arr = (_lib.AdamWGroup * len(chunk))(*[e[0] for e in chunk])
             stream = C.c_void_p(torch.cuda.current_stream(chunk[0][1]).cuda_stream)
             if norm is not None:
-                fn, value = (self._lib.cinema_adamw_step_clipped, norm) if wide is None else (self._lib.cinema_adamw_step_clipped_f64, wide)
-                _lib.check(fn(arr, len(chunk), int(self.clear_grads), value.data_ptr(), self.max_grad_norm, stream), "cinema_adamw_step_clipped")
+                fn = self._lib.cinema_adamw_step_clipped_f64 if norm.dtype == torch.float64 else self._lib.cinema_adamw_step_clipped
+                _lib.check(fn(arr, len(chunk), int(self.clear_grads), norm.data_ptr(), self.max_grad_norm, stream), "cinema_adamw_step_clipped")
                 continue
             fn = self._lib.cinema_adamw_step_clear if self.clear_grads else self._lib.cinema_adamw_step
             _lib.check(fn(arr, len(chunk), stream), "cinema_adamw_step")

@@ -427,8 +427,7 @@ class HotPathTrainer:
                 w.wait()
         if clipped:
             of = lambda opt: _lib.binding().grad_norm_wide([p.grad for g in opt.param_groups for p in g["params"] if p.grad is not None], 2.0)[1].to(self.device)
-            wide = par.union_grad_norm(of(self.opt_local), None if self.opt_mlp is None else of(self.opt_mlp), self.pg)
-            norm = (wide.float(), wide)
+            norm = par.union_grad_norm(of(self.opt_local), None if self.opt_mlp is None else of(self.opt_mlp), self.pg)
             self.opt_local.step(grad_norm=norm)
         if self.opt_mlp is not None:
             self.opt_mlp.step(grad_norm=norm)

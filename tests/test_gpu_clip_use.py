@@ -95,22 +95,25 @@ def test_clipped_update_where_the_norm_leaves_fp32(n):
     assert float((got[1] - got[0]).abs().max()) <= 0.125 * 2.0 ** -19
 
 
-def test_a_given_norm_as_a_pair():
-    """fp32 and 64 bits: the 64-bit one clips; both have to be there, on the gradients' device"""
+def test_a_given_norm_in_either_type():
+    """fp32 and fp64 values clip, also the union norm as it comes; anything else is refused and changes nothing"""
     from cinema_amd import _lib
+    from cinema_amd import parallel as par
     from cinema_amd.optim import HipAdamW
     outs = []
-    for given in (lambda n: None, lambda n: n.float(), lambda n: (n.float(), n)):
+    for given in (lambda n: None, lambda n: n.float(), lambda n: n, lambda n: par.union_grad_norm(n.float(), None)):
         (p,) = params(torch.linspace(-1, 1, 77, device="cuda"))
         opt = HipAdamW([p], lr=0.1, max_grad_norm=0.25)
-        opt.step(grad_norm=given(p.grad.double().norm()))
-        assert opt.grad_norm.dtype == torch.float32 and opt.grad_norm.dim() == 0
+        n = p.grad.double().norm()
+        opt.step(grad_norm=given(n))
+        assert opt.grad_norm.dtype == torch.float32 and opt.grad_norm.dim() == 0 and abs(float(opt.grad_norm) - float(n)) <= float(n) * 2.0 ** -22
         outs.append(p.detach().clone())
     assert all(float((o - outs[0]).abs().max()) <= 0.1 * 2.0 ** -18 for o in outs)
-    one = torch.ones((), device="cuda")
-    for bad in [(one, one), (one, one.double().cpu()), (one.double(), one.double()), (one, torch.ones(2, device="cuda").double())]:
+    one, kept = torch.ones((), device="cuda"), opt.grad_norm
+    for bad in [one.half(), one.long(), one.cpu(), one.double().cpu(), torch.ones(2, device="cuda"), torch.ones(2, device="cuda").double()]:
         with pytest.raises(_lib.CinemaHipError, match="grad_norm"):
             opt.step(grad_norm=bad)
+    assert opt.grad_norm is kept and opt.state[p]["step"] == 1
 
 
 def test_no_gradients_have_the_norm_0_where_the_parameters_are():
